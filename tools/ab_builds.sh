@@ -16,7 +16,7 @@ if [ "$MODE" = build ]; then
     ( cd yolo2_light_amd/csrc
       case $v in ''|*[!0-9]*) fl_var=ABFLAGS_$v; FL=${!fl_var};; *) FL="-DYL_LAB -DX_DBG=$v";; esac
       SLP=""; [ "$SRC" = conv_f32_wino32 ] && SLP="-fno-slp-vectorize"       # as csrc/Makefile builds that file
-      /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off $SLP $FL -c $SRC.hip -o build_repro/${SRC}_x$v.o
+      /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops $SLP $FL -c $SRC.hip -o build_repro/${SRC}_x$v.o
       objs=$(ls build/*.o | grep -v "build/$SRC.o")
       /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o ../../tools/ab/libyolo2hip_x$v.so $objs build_repro/${SRC}_x$v.o -ldl -lpthread )
     echo "built tools/ab/libyolo2hip_x$v.so"

@@ -5,7 +5,7 @@ set -e
 cd /root/repo/yolo2_light_amd/csrc
 stem=$1; shift
 mkdir -p /tmp/kbuild
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function "$@" -c $stem.hip -o /tmp/kbuild/$stem.o -save-temps=obj
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $stem.hip -o /tmp/kbuild/$stem.o -save-temps=obj
 python3 - "$stem" <<'PY'
 import re,sys
 s=open('/tmp/kbuild/%s-hip-amdgcn-amd-amdhsa-gfx950.s'%sys.argv[1]).read()
