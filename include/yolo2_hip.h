@@ -454,6 +454,84 @@ int yl_network_calibrate(yl_network *net, const float *images_host, int n_images
 float yl_entropy_from_histogram(const uint32_t *counts, int max_bin, float bin_width);
 
 /* ------------------------------------------------------------------ *
+ *  MXFP4 operators (new): microscaled 4-bit floating point -- rounding, products, the linear layer, the convolution.
+ *  The reference's smallest multiply-add formats are INT8 (src/yolov2_forward_network_quantized.c:527) and one bit
+ *  (src/yolov2_forward_network.c:116); these run on the scaled FP4 matrix instruction, 4 bits and 1/32 byte of scale a value.
+ *
+ *  Every entry takes the device its pointers belong to and a stream of that device (hipStream_t as void *, NULL = the
+ *  default stream), is asynchronous on it, leaves the caller's current device as it was, keeps no state between calls and
+ *  allocates nothing, so calls from several threads, streams and captured graphs do not meet.  All data pointers are device
+ *  memory.  A call that returns an error has launched nothing.
+ * ------------------------------------------------------------------ */
+
+/* element types of the ordinary tensors these entries read and write */
+enum { YL_F32 = 0, YL_F16 = 1, YL_BF16 = 2 };
+
+/* rows x k values in MXFP4.  A row is cut into blocks of 32 values along k; block j of row r holds
+ *   codes [(r * ld + j) * 16 .. + 15]   32 E2M1 codes (sign, 2 exponent bits, 1 mantissa bit: 0 .5 1 1.5 2 3 4 6), value 2i in the
+ *                                       low half of byte i, value 2i + 1 in the high half
+ *   scales[r * ld + j]                  E8M0: the block's values are code * 2^(scale - 127); 255 = every value of the block is NaN
+ * ld >= ceil(k / 32) is the row stride in blocks (a multiple of 4 keeps rows on 64 bytes and lets kernels load scales by words).
+ * Where k % 32 != 0 the codes behind k in a row's last block are zero.  Blocks from ceil(k / 32) to ld are neither read nor written.
+ * codes must be 16-byte aligned. */
+typedef struct yl_mx_matrix {
+    void *codes, *scales;
+    int64_t rows, k, ld;
+} yl_mx_matrix;
+
+/* batch x rows x k ordinary values, element (b, r, i) at data + (b * batch_stride + r * row_stride + i * k_stride) elements.
+ * A row-major matrix: batch = 1, k_stride = 1.  An NCHW map read as one row of channels a pixel: rows = H * W, k = C,
+ * batch_stride = C * H * W, row_stride = 1, k_stride = H * W. */
+typedef struct yl_dense {
+    void *data;
+    int type;                                    /* YL_F32 / YL_F16 / YL_BF16 */
+    int64_t batch, rows, k;
+    int64_t batch_stride, row_stride, k_stride;  /* elements, >= 0 */
+} yl_dense;
+
+/* what follows a product: y = activate(sum + bias[n]) + residual, in 32 bits, rounded once to y's type */
+typedef struct yl_mx_epilogue {
+    const float *bias;          /* one a column of w / filter, or NULL */
+    int activation;             /* YL_LINEAR, YL_LEAKY, ... (any activation of this header) */
+    const void *residual;       /* y's type and shape, or NULL; may be y itself, may not otherwise overlap it */
+    int64_t residual_stride;    /* elements from row to row (the convolution: ignored, y's layout) */
+} yl_mx_epilogue;
+
+/* a row stride for k values: ceil(k / 32) rounded up to a multiple of 4 */
+int64_t yl_mx_blocks(int64_t k);
+
+/* src -> dst, dst->rows == src->batch * src->rows, dst->k == src->k.  For every block, with m = the largest magnitude in it:
+ * scale = 2^(floor(log2 m) - 2), not below 2^-127; codes = value / scale rounded to the nearest, ties to the even code, magnitudes
+ * above 6 become 6.  A block that holds an Inf or a NaN becomes NaN as a whole (scale 255, codes 0). */
+int yl_mx_quantize(int device, void *stream, const yl_dense *src, const yl_mx_matrix *dst);
+
+/* the values that src stands for, rounded to dst->type (FP32 and BF16 hold everything yl_mx_quantize makes exactly) */
+int yl_mx_dequantize(int device, void *stream, const yl_mx_matrix *src, const yl_dense *dst);
+
+/* y[m][n] = activate(sum over k of x[m][k] * w[n][k] + bias[n]) + residual[m][n], summed in 32 bits.
+ * y: batch 1, rows = x->rows, k = w->rows, k_stride 1; it may not overlap the operands. */
+int yl_mx_matmul(int device, void *stream, const yl_mx_matrix *x, const yl_mx_matrix *w, const yl_mx_epilogue *epilogue, const yl_dense *y);
+
+/* yl_mx_matmul on yl_mx_quantize(x), the same bits, in one call.  x: batch 1.  `workspace` is device memory of at least
+ * yl_mx_linear_workspace(x->rows, x->k) bytes, 16-byte aligned, which holds the rounded x while the call runs: calls that may run
+ * at the same time need one each.  (It is 0 where the product rounds x itself: a few rows, the single token of a decoding step.) */
+int64_t yl_mx_linear_workspace(int64_t rows, int64_t k);
+int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix *w, const yl_mx_epilogue *epilogue, const yl_dense *y,
+                 void *workspace, int64_t workspace_bytes);
+
+/* A convolution over a map in MXFP4, one row of channels a pixel: x->rows = batch * h * w in the order (b, y, x), x->k = channels.
+ * filters: one row a filter, the taps (ky, kx) one after the other, each with its channels padded by zeros to whole blocks:
+ * filters->k = size * size * ceil(channels / 32) * 32.
+ * out (float [batch][filters][oh][ow], NULL if not wanted) = activate(convolution + bias) + residual (the same layout);
+ * q_out (NULL if not wanted): the same values rounded to MXFP4 as the next layer's x, rows = batch * oh * ow, k = filters.
+ * oh = (h + 2 * pad - size) / stride + 1, ow likewise; size <= 5. */
+typedef struct yl_mx_conv {
+    int batch, h, w, size, stride, pad;
+} yl_mx_conv;
+int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_matrix *filters, const yl_mx_conv *shape,
+                 const yl_mx_epilogue *epilogue, float *out, const yl_mx_matrix *q_out);
+
+/* ------------------------------------------------------------------ *
  *  Several GPUs of one node, ONE host process (new).  The reference selects a single
  *  device (`-i <n>` -> cuda_set_device, src/main.c:653-661) and hands network_predict the whole batch;
  *  a group splits that batch of independent images over the listed devices (weights replicated, one

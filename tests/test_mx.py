@@ -1,0 +1,219 @@
+"""The MXFP4 entries without a GPU: the 64-bit oracle against the format's own statements, and every refusal.  (A refused call has
+launched nothing and touched no pointer, so the pointers here are numbers; accepted arguments end at the missing device.)"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import mx_oracle as o
+from yolo2_light_amd._lib import Dense, MxConv, MxEpilogue, MxMatrix, lib, last_error
+
+ARG, DEVICE = -1, -4
+F32, F16, BF16 = 0, 1, 2
+HAVE_GPU = lib.yl_device_count() > 0
+MB = 1 << 20
+
+
+# ------------------------------------------------------------------ the oracle
+def test_oracle_rounds_to_the_nearest_code_with_ties_to_even():
+    x = np.array([[6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 0.26, 0.74, -0.25, -0.75, 7.9, -7.9, 5.01, 4.99] + [0.0] * 16])
+    code, scale = o.quantize(x)
+    assert scale[0, 0] == 127                                          # floor(log2 7.9) = 2
+    assert o.values(code, scale, 16)[0].tolist() == [6, 0, 1, 1, 2, 2, 4, 4, .5, .5, 0, -1, 6, -6, 6, 4]
+
+
+def test_oracle_scales():
+    for top, byte in ((1.0, 125), (1.999, 125), (2.0, 126), (4.0, 127), (2.0 ** -125, 0), (2.0 ** -149, 0), (2.0 ** 127, 252), (0.0, 0), (np.inf, 255), (np.nan, 255)):
+        x = np.zeros((1, 32))
+        x[0, 7] = top
+        assert o.quantize(x)[1][0, 0] == byte, top
+
+
+def test_oracle_pack_is_unpacked():
+    code = np.arange(64, dtype=np.uint8).reshape(1, 64) % 16
+    assert (o.unpack(o.pack(code))[0] == code[0]).all()
+    assert o.pack(code)[0, 0] == 0x10
+
+
+# ------------------------------------------------------------------ refusals
+def matrix(rows=4, k=64, ld=4, codes=16 * MB, scales=32 * MB):
+    return MxMatrix(codes, scales, rows, k, ld)
+
+
+def dense(rows=4, k=64, type=F32, data=48 * MB, batch=1, bs=0, rs=None, ks=1):
+    return Dense(data, type, batch, rows, k, bs, k if rs is None else rs, ks)
+
+
+def r(x):
+    return None if x is None else C.byref(x)
+
+
+def quantize(src, dst, device=0):
+    return lib.yl_mx_quantize(device, None, r(src), r(dst))
+
+
+def dequantize(src, dst, device=0):
+    return lib.yl_mx_dequantize(device, None, r(src), r(dst))
+
+
+X, W, Y = dict(rows=4, k=64, ld=4), dict(rows=8, k=64, ld=4, codes=64 * MB, scales=80 * MB), dict(rows=4, k=8, data=96 * MB)
+
+
+def matmul(x=X, w=W, y=Y, e=None, device=0):
+    x, w, y = matrix(**x) if x else None, matrix(**w) if w else None, dense(**y) if y else None
+    return lib.yl_mx_matmul(device, None, r(x), r(w), r(e), r(y))
+
+
+def linear(x=None, w=W, y=Y, e=None, ws=112 * MB, ws_bytes=MB, device=0):
+    x = dense() if x is None else x
+    return lib.yl_mx_linear(device, None, r(x), r(matrix(**w)), r(e), r(dense(**y)), ws, ws_bytes)
+
+
+def refused(rc, what):
+    assert rc == ARG and what in last_error(), (rc, last_error())
+
+
+def accepted(rc):
+    assert rc == DEVICE and "no HIP device" in last_error(), (rc, last_error())
+
+
+def test_blocks():
+    assert [lib.yl_mx_blocks(k) for k in (0, 1, 32, 33, 128, 129, 4096)] == [0, 4, 4, 4, 4, 8, 128]
+    assert lib.yl_mx_blocks(-1) == 0 and lib.yl_mx_blocks(1 << 60) == 0
+
+
+def test_linear_workspace_is_whole_rows_or_nothing():
+    for rows, k in ((1, 1), (1, 4096), (300, 33), (5000, 4096)):
+        need = lib.yl_mx_linear_workspace(rows, k)
+        assert need in (0, rows * lib.yl_mx_blocks(k) * 17)
+    assert lib.yl_mx_linear_workspace(5000, 4096) > 0
+    assert lib.yl_mx_linear_workspace(0, 64) == 0 and lib.yl_mx_linear_workspace(4, 0) == 0
+
+
+@pytest.mark.parametrize("change, what", [
+    (dict(rows=-1), "negative"), (dict(k=-1), "negative"), (dict(k=129), "ld"), (dict(ld=(1 << 20) + 1), "ld"), (dict(codes=None), "NULL"),
+    (dict(scales=None), "NULL"), (dict(codes=16 * MB + 8), "16-byte"), (dict(rows=1 << 45), "too large")])
+def test_refused_matrices(change, what):
+    m = {**dict(rows=4, k=64, ld=4), **change}
+    refused(quantize(dense(), matrix(**m)), what)
+    refused(dequantize(matrix(**m), dense()), what)
+    refused(matmul(x=m), what)
+    refused(matmul(w={**W, **change}), what)
+
+
+@pytest.mark.parametrize("change, what", [
+    (dict(type=3), "type"), (dict(type=-1), "type"), (dict(rows=-1), "negative"), (dict(k=-2), "negative"), (dict(rs=-1), "negative"), (dict(ks=-1), "negative"),
+    (dict(batch=-1), "negative"), (dict(data=None), "NULL"), (dict(data=48 * MB + 2), "aligned"), (dict(data=48 * MB + 1, type=F16), "aligned"),
+    (dict(rs=1 << 50), "too large"), (dict(rows=1 << 30, rs=1 << 40), "too large")])
+def test_refused_tensors(change, what):
+    refused(quantize(dense(**change), matrix()), what)
+    refused(dequantize(matrix(), dense(**change)), what)
+    refused(linear(x=dense(**change)), what)
+
+
+def test_refused_shapes_and_overlaps_of_rounding():
+    refused(quantize(None, matrix()), "NULL")
+    refused(quantize(dense(), None), "NULL")
+    refused(quantize(dense(rows=5), matrix()), "batch * rows by k")
+    refused(quantize(dense(k=63), matrix()), "batch * rows by k")
+    refused(quantize(dense(batch=2, rows=4), matrix(rows=4)), "batch * rows by k")
+    refused(quantize(dense(data=16 * MB), matrix()), "overlaps")
+    refused(quantize(dense(data=32 * MB), matrix()), "overlaps")
+    refused(quantize(dense(), matrix(scales=16 * MB + 16)), "overlap")
+    refused(dequantize(matrix(), dense(data=16 * MB)), "overlaps")
+    refused(dequantize(matrix(), dense(rs=63)), "overlap")             # two rows of the result share a place
+    refused(dequantize(matrix(), dense(rs=0)), "overlap")
+    refused(dequantize(matrix(rows=8), dense(batch=2, bs=64)), "overlap")
+    if not HAVE_GPU:
+        accepted(quantize(dense(rs=0), matrix()))                      # a broadcast input may
+        accepted(quantize(dense(rows=4, k=64, rs=1, ks=4), matrix()))
+        accepted(dequantize(matrix(), dense(rs=1, ks=4)))
+        accepted(quantize(dense(rows=0), matrix(rows=0)))
+
+
+def test_refused_products():
+    refused(matmul(x=None), "NULL")
+    refused(matmul(w=None), "NULL")
+    refused(matmul(y=None), "NULL")
+    refused(matmul(w={**W, "k": 65}), "k differ")
+    refused(matmul(y={**Y, "rows": 5}), "rows")
+    refused(matmul(y={**Y, "k": 9}), "rows")
+    refused(matmul(y={**Y, "batch": 2}), "batch")
+    refused(matmul(y={**Y, "ks": 2, "rs": 16}), "k_stride")
+    refused(matmul(y={**Y, "rs": 7}), "overlap")
+    refused(matmul(y={**Y, "data": 16 * MB}), "overlaps x")
+    refused(matmul(y={**Y, "data": 80 * MB}), "overlaps w")
+    for e, what in ((MxEpilogue(None, 13, None, 0), "activation"), (MxEpilogue(None, -1, None, 0), "activation"), (MxEpilogue(2, 3, None, 0), "bias"),
+                    (MxEpilogue(96 * MB, 3, None, 0), "bias"), (MxEpilogue(None, 3, 96 * MB + 4, 8), "residual"), (MxEpilogue(None, 3, 96 * MB, 16), "residual"),
+                    (MxEpilogue(None, 3, 200 * MB, -1), "residual"), (MxEpilogue(None, 3, 200 * MB + 2, 8), "residual")):
+        refused(matmul(e=e), what)
+    if not HAVE_GPU:
+        accepted(matmul(e=MxEpilogue(None, 3, 96 * MB, 8)))            # the residual may be y itself
+        accepted(matmul(e=MxEpilogue(128 * MB, 7, 200 * MB, 8)))
+        accepted(matmul(x={**X, "rows": 0, "codes": None, "scales": None}, y={**Y, "rows": 0, "data": None}))
+        accepted(matmul(x={**X, "k": 0, "ld": 0, "codes": None, "scales": None}, w={**W, "k": 0, "ld": 0}))
+
+
+def test_refused_linear_layers():
+    big, wide = dict(rows=5000, k=64), {**Y, "rows": 5000}
+    refused(linear(x=dense(batch=2, bs=256)), "batch")
+    refused(linear(x=dense(k=63)), "k differ")
+    refused(linear(x=dense(data=96 * MB)), "overlaps x")
+    refused(linear(x=dense(**big), y=wide, ws=None), "workspace")
+    refused(linear(x=dense(**big), y=wide, ws_bytes=100), "workspace")
+    refused(linear(x=dense(**big), y=wide, ws=112 * MB + 8), "aligned")
+    for at in (48, 64, 80, 96):
+        refused(linear(x=dense(**big), y=wide, ws=at * MB), "overlaps")
+    refused(linear(x=dense(**big), y=wide, e=MxEpilogue(112 * MB, 3, None, 0)), "overlaps")
+    refused(linear(x=dense(**big), y=wide, e=MxEpilogue(None, 3, 112 * MB, 8)), "overlaps")
+    if not HAVE_GPU:
+        accepted(linear())
+        accepted(linear(x=dense(**big), y=wide))
+
+
+def conv(x=None, f=None, shape=(1, 4, 4, 3, 1, 1), e=None, out=96 * MB, q=None, device=0):
+    x = matrix(rows=16, k=32, ld=1) if x is None else x
+    f = matrix(rows=8, k=9 * 32, ld=12, codes=64 * MB, scales=80 * MB) if f is None else f
+    return lib.yl_mx_conv2d(device, None, r(x), r(f), r(MxConv(*shape)) if shape else None, r(e), out, r(q))
+
+
+def test_refused_convolutions():
+    refused(conv(shape=None), "NULL")
+    for shape in ((1, 4, 4, 0, 1, 0), (1, 4, 4, 6, 1, 1), (1, 4, 4, 3, 0, 1), (1, 4, 4, 3, 1, -1), (1, 4, 4, 3, 1, 3), (-1, 4, 4, 3, 1, 1), (1, 0, 4, 3, 1, 1)):
+        refused(conv(shape=shape), "shape")
+    refused(conv(shape=(1, 4, 5, 3, 1, 1)), "batch * h * w")
+    refused(conv(x=matrix(rows=16, k=33, ld=4)), "filters' k")
+    refused(conv(x=matrix(rows=16, k=0, ld=0)), "no channels")
+    refused(conv(x=matrix(rows=4, k=32, ld=1), shape=(1, 2, 2, 3, 1, 0)), "larger")
+    refused(conv(out=96 * MB + 2), "aligned")
+    for at in (16, 32, 64, 80):
+        refused(conv(out=at * MB), "overlaps")
+    refused(conv(e=MxEpilogue(96 * MB, 3, None, 0)), "bias")
+    refused(conv(e=MxEpilogue(None, 3, 96 * MB + 4, 0)), "residual")
+    q = dict(rows=16, k=8, ld=1, codes=112 * MB, scales=128 * MB)
+    refused(conv(q=matrix(**{**q, "rows": 15})), "q_out")
+    refused(conv(q=matrix(**{**q, "k": 9})), "q_out")
+    for at in (16, 32, 64, 80, 96):
+        refused(conv(q=matrix(**{**q, "codes": at * MB})), "q_out overlaps")
+    if not HAVE_GPU:
+        accepted(conv())
+        accepted(conv(q=matrix(**q)))
+        accepted(conv(out=None, q=matrix(**q)))
+        accepted(conv(e=MxEpilogue(None, 3, 96 * MB, 0)))
+        accepted(conv(x=matrix(rows=0, k=32, ld=1), shape=(0, 4, 4, 3, 1, 1)))
+
+
+def test_no_such_device():
+    for device in (-1, 4096):
+        rc = quantize(dense(), matrix(), device=device)
+        assert rc == (ARG if HAVE_GPU else DEVICE), last_error()
+
+
+def test_python_refuses_what_is_not_on_a_gpu():
+    torch = pytest.importorskip("torch")
+    from yolo2_light_amd import YoloHipError, mx
+    x = torch.zeros(4, 64)
+    for call in (lambda: mx.quantize(x), lambda: mx.quantize_nchw(x), lambda: mx.quantize_filters(x), lambda: mx.linear(x, None),
+                 lambda: mx.Matrix(x, x, 64), lambda: mx.matmul(x, x), lambda: mx.conv2d(x, x, 1, 2, 2, 1), lambda: mx.dequantize(x)):
+        with pytest.raises(YoloHipError):
+            call()

@@ -57,6 +57,30 @@ class LayerDesc(C.Structure):
 
 _vp = C.c_void_p
 
+
+class MxMatrix(C.Structure):
+    """struct yl_mx_matrix."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("k", C.c_int64), ("ld", C.c_int64)]
+
+
+class Dense(C.Structure):
+    """struct yl_dense."""
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("batch", C.c_int64), ("rows", C.c_int64), ("k", C.c_int64),
+                ("batch_stride", C.c_int64), ("row_stride", C.c_int64), ("k_stride", C.c_int64)]
+
+
+class MxEpilogue(C.Structure):
+    """struct yl_mx_epilogue."""
+    _fields_ = [("bias", C.c_void_p), ("activation", C.c_int), ("residual", C.c_void_p), ("residual_stride", C.c_int64)]
+
+
+class MxConv(C.Structure):
+    """struct yl_mx_conv."""
+    _fields_ = [("batch", C.c_int), ("h", C.c_int), ("w", C.c_int), ("size", C.c_int), ("stride", C.c_int), ("pad", C.c_int)]
+
+
+_mxp, _dnp, _epp = C.POINTER(MxMatrix), C.POINTER(Dense), C.POINTER(MxEpilogue)
+
 ABI_VERSION = 4          # YL_ABI_VERSION of the include/yolo2_hip.h this table was written against
 
 _SIGS = {
@@ -131,6 +155,13 @@ _SIGS = {
     "yl_entropy_from_histogram": (C.c_float, [C.POINTER(C.c_uint32), C.c_int, C.c_float]),
     "yl_network_get_boxes_batch": (C.c_int, [_vp, c_int_p, c_int_p, C.c_float, C.c_int, C.c_int, C.c_float, C.c_int,
                                              c_float_p, c_int_p]),
+    "yl_mx_blocks": (C.c_int64, [C.c_int64]),
+    "yl_mx_quantize": (C.c_int, [C.c_int, _vp, _dnp, _mxp]),
+    "yl_mx_dequantize": (C.c_int, [C.c_int, _vp, _mxp, _dnp]),
+    "yl_mx_matmul": (C.c_int, [C.c_int, _vp, _mxp, _mxp, _epp, _dnp]),
+    "yl_mx_linear_workspace": (C.c_int64, [C.c_int64, C.c_int64]),
+    "yl_mx_linear": (C.c_int, [C.c_int, _vp, _dnp, _mxp, _epp, _dnp, _vp, C.c_int64]),
+    "yl_mx_conv2d": (C.c_int, [C.c_int, _vp, _mxp, _mxp, C.POINTER(MxConv), _epp, _vp, _mxp]),
     "yl_shard_range": (C.c_int, [C.c_int, C.c_int, C.c_int, c_int_p, c_int_p]),
     "yl_group_create": (C.c_int, [_vp, c_int_p, C.c_int, C.POINTER(_vp)]),
     "yl_group_destroy": (None, [_vp]),

@@ -1,0 +1,59 @@
+// mx_device.h -- what the MXFP4 kernels share on the device.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include "../../include/yolo2_hip.h"
+
+namespace yl {
+
+typedef int mx_v4i __attribute__((ext_vector_type(4)));
+typedef int mx_v8i __attribute__((ext_vector_type(8)));
+typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
+typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
+typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
+
+// one value of an ordinary tensor <-> FP32.  To FP16 / BF16: nearest even, half a step (2^-11 / 2^-8 of the value) at most.
+template <int TYPE>
+__device__ __forceinline__ float mx_load(const void *p, int64_t i)
+{
+    if constexpr (TYPE == YL_F32) return reinterpret_cast<const float *>(p)[i];
+    else if constexpr (TYPE == YL_F16) return (float)reinterpret_cast<const _Float16 *>(p)[i];
+    else return __builtin_bit_cast(float, (unsigned)reinterpret_cast<const unsigned short *>(p)[i] << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ void mx_store(void *p, int64_t i, float v)
+{
+    if constexpr (TYPE == YL_F32) reinterpret_cast<float *>(p)[i] = v;
+    else if constexpr (TYPE == YL_F16) reinterpret_cast<_Float16 *>(p)[i] = (_Float16)v;
+    else reinterpret_cast<__bf16 *>(p)[i] = (__bf16)v;
+}
+
+// The scale byte of a block whose largest magnitude has the FP32 bits `top` (exponent field f): floor(log2) is f - 127, the largest
+// E2M1 exponent is 2, so the byte is f - 2, not below 0 (2^-127; subnormals and zero have f = 0).  f = 255 is an Inf or a NaN.
+__device__ __forceinline__ unsigned mx_scale_byte(unsigned top)
+{
+    const unsigned f = top >> 23;
+    return f == 255 ? 255u : (f > 2 ? f - 2 : 0u);
+}
+// eight values / 2^(byte - 127) -> eight codes: nearest even, saturated at 6 (v_cvt_scalef32_pk_fp4_f32 reads the scale's exponent
+// field alone, byte 0 included).  Dividing by a power of two is exact here: |value| < 8 * scale.
+__device__ __forceinline__ unsigned mx_codes8(const float *v, unsigned byte)
+{
+    const float s = __builtin_bit_cast(float, byte << 23);
+    unsigned q = 0;
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], s, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[2], v[3], s, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[4], v[5], s, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], s, 3);
+    return q;
+}
+__device__ __forceinline__ unsigned mx_abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+
+__device__ __forceinline__ mx_v8i mx_operand(mx_v4i c) { return mx_v8i{c[0], c[1], c[2], c[3], 0, 0, 0, 0}; }
+
+// magnitude bits' maximum sorts NaN above Inf above every number, as unsigned integers do
+
+}  // namespace yl

@@ -1,0 +1,256 @@
+"""MXFP4 operators on torch tensors of a GPU: the yl_mx_* entries of include/yolo2_hip.h (formats and formulas stand there).
+
+    q = mx.quantize(x)                         # [..., k] FP32 / FP16 / BF16 -> Matrix (one row a k-vector)
+    y = mx.matmul(q, w, bias=b, activation="leaky")
+    y = mx.linear(x, w, bias=b)                # == matmul(quantize(x), w), in one call
+    f = mx.quantize_filters(weights)           # [n, c, size, size] -> Matrix
+    y = mx.conv2d(mx.quantize_nchw(x), f, batch, h, w, size, stride, pad, bias=b, activation="leaky", residual=r)
+
+Every call runs on the current stream of its tensors' device and returns without waiting.  There is no backward pass: a call on a
+tensor that requires a gradient raises.  Plumbing only: all arithmetic happens in libyolo2hip.so."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from ._lib import Dense, MxConv, MxEpilogue, MxMatrix, YoloHipError, lib, check
+
+BLOCK = 32
+ACTIVATIONS = {"logistic": 0, "relu": 1, "relie": 2, "linear": 3, "ramp": 4, "tanh": 5, "plse": 6, "leaky": 7, "elu": 8, "loggy": 9,
+               "stair": 10, "hardtan": 11, "lhtan": 12}
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ref = C.byref
+
+
+def _fail(what: str):
+    raise YoloHipError("mx: " + what)
+
+
+def _tensor(t, name: str, device=None):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        _fail("%s is not a tensor on a GPU" % name)
+    if device is not None and t.device != device:
+        _fail("%s is on %s, not on %s" % (name, t.device, device))
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail("%s requires a gradient, and there is no backward pass: detach it, or call under torch.no_grad()" % name)
+    return t
+
+
+def _type(t, name: str) -> int:
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        _fail("%s is %s: float32, float16 and bfloat16 are taken" % (name, t.dtype))
+    return code
+
+
+class Matrix:
+    """rows x k values in MXFP4: codes uint8 [rows, 16 * ld], scales uint8 [rows, ld], ld >= ceil(k / 32) blocks a row."""
+    __slots__ = ("codes", "scales", "k", "_c")
+
+    def __init__(self, codes, scales, k: int):
+        self.codes, self.scales, self.k = _tensor(codes, "codes"), _tensor(scales, "scales", codes.device), int(k)
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
+            _fail("codes and scales are two-dimensional uint8 tensors")
+        rows, ld = scales.shape
+        if codes.shape[0] != rows or codes.shape[1] != 16 * ld or not codes.is_contiguous() or not scales.is_contiguous():
+            _fail("codes [rows, 16 * ld] and scales [rows, ld] are contiguous and of the same rows and blocks")
+        if self.k < 0 or ld < (self.k + BLOCK - 1) // BLOCK:
+            _fail("k = %d needs %d blocks, the matrix has %d" % (self.k, (self.k + BLOCK - 1) // BLOCK, ld))
+        self._c = MxMatrix(codes.data_ptr(), scales.data_ptr(), rows, self.k, ld)
+
+    @classmethod
+    def empty(cls, rows: int, k: int, device) -> "Matrix":
+        ld = lib.yl_mx_blocks(k)
+        return cls(torch.empty(rows, 16 * ld, dtype=torch.uint8, device=device), torch.empty(rows, ld, dtype=torch.uint8, device=device), k)
+
+    @property
+    def rows(self) -> int:
+        return self.scales.shape[0]
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def _matrix(m, name: str, device=None) -> Matrix:
+    if not isinstance(m, Matrix):
+        _fail("%s is not an mx.Matrix" % name)
+    if device is not None and m.codes.device != device:
+        _fail("%s is on %s, not on %s" % (name, m.codes.device, device))
+    return m
+
+
+def _at(device):
+    return device.index, torch.cuda.current_stream(device).cuda_stream
+
+
+def _rows_of(x, name: str) -> Dense:
+    """[..., k] as rows of k: the leading axes have to be one run of equal steps."""
+    kind = _type(x, name)
+    if x.dim() == 0:
+        _fail("%s has no axis" % name)
+    if x.dim() == 2:
+        rows, step = x.shape[0], x.stride(0)
+    elif x.dim() == 1:
+        rows, step = 1, 0
+    else:
+        try:
+            flat = x.view(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1])
+        except RuntimeError:
+            _fail("the leading axes of %s cannot be taken as one axis of rows: make it contiguous" % name)
+        rows, step = flat.shape[0], flat.stride(0)
+    return Dense(x.data_ptr(), kind, 1, rows, x.shape[-1], 0, step, x.stride(-1))
+
+
+def _map_of(x, name: str) -> Dense:
+    """[batch, c, h, w] as one row of channels a pixel."""
+    kind = _type(x, name)
+    if x.dim() != 4:
+        _fail("%s is not [batch, channels, h, w]" % name)
+    b, c, h, w = x.shape
+    if h > 1 and w > 1 and x.stride(2) != w * x.stride(3):
+        _fail("rows of the map %s do not follow one another: make it contiguous" % name)
+    return Dense(x.data_ptr(), kind, b, h * w, c, x.stride(0), x.stride(3) if w > 1 else x.stride(2), x.stride(1))
+
+
+def _quantize(src: Dense, device, out: Optional[Matrix]) -> Matrix:
+    rows = src.batch * src.rows
+    if out is None:
+        out = Matrix.empty(rows, src.k, device)
+    check(lib.yl_mx_quantize(*_at(device), _ref(src), _ref(_matrix(out, "out", device)._c)), "yl_mx_quantize")
+    return out
+
+
+def quantize(x, out: Optional[Matrix] = None) -> Matrix:
+    """x [..., k], any strides -> Matrix of x.numel() / k rows."""
+    _tensor(x, "x")
+    return _quantize(_rows_of(x, "x"), x.device, out)
+
+
+def quantize_nchw(x, out: Optional[Matrix] = None) -> Matrix:
+    """A map [batch, c, h, w] -> Matrix of batch * h * w rows of c values (conv2d's x)."""
+    _tensor(x, "x")
+    return _quantize(_map_of(x, "x"), x.device, out)
+
+
+def quantize_filters(w) -> Matrix:
+    """Filters [n, c, size, size] -> Matrix of n rows, tap after tap, the channels of each padded by zeros to whole blocks."""
+    _tensor(w, "w")
+    if w.dim() != 4 or w.shape[2] != w.shape[3]:
+        _fail("w is not [filters, channels, size, size]")
+    n, c, size, _ = w.shape
+    rows = torch.zeros(n, size, size, (c + BLOCK - 1) // BLOCK * BLOCK, dtype=w.dtype, device=w.device)
+    rows[..., :c] = w.permute(0, 2, 3, 1)
+    return quantize(rows.view(n, -1))
+
+
+def _dequantize(q: Matrix, out, dst: Dense):
+    check(lib.yl_mx_dequantize(*_at(q.device), _ref(q._c), _ref(dst)), "yl_mx_dequantize")
+    return out
+
+
+def dequantize(q: Matrix, dtype=torch.float32, out=None):
+    """The values of q, [rows, k]."""
+    _matrix(q, "q")
+    if out is None:
+        out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
+    return _dequantize(q, out, _rows_of(_tensor(out, "out", q.device), "out"))
+
+
+def dequantize_nchw(q: Matrix, batch: int, h: int, w: int, dtype=torch.float32, out=None):
+    """The values of a quantised map, [batch, q.k, h, w]."""
+    _matrix(q, "q")
+    if out is None:
+        out = torch.empty(batch, q.k, h, w, dtype=dtype, device=q.device)
+    return _dequantize(q, out, _map_of(_tensor(out, "out", q.device), "out"))
+
+
+def _epilogue(n: int, device, bias, activation, residual) -> Optional[MxEpilogue]:
+    act = ACTIVATIONS.get(activation) if isinstance(activation, str) else activation
+    if act is None or not isinstance(act, int):
+        _fail("unknown activation %r" % (activation,))
+    if bias is not None:
+        _tensor(bias, "bias", device)
+        if bias.dtype is not torch.float32 or bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous():
+            _fail("bias is a contiguous float32 tensor of %d values" % n)
+    if bias is None and residual is None and act == 3:
+        return None
+    return MxEpilogue(bias.data_ptr() if bias is not None else None, act, residual.data_ptr() if residual is not None else None,
+                      residual.stride(0) if residual is not None else 0)
+
+
+def _linear_args(lead, m: int, w: Matrix, device, bias, activation, residual, dtype, out):
+    n = w.rows
+    if out is None:
+        out = torch.empty(*lead, n, dtype=dtype, device=device)
+    elif tuple(out.shape) != (*lead, n):
+        _fail("out is not %s" % ((*lead, n),))
+    y = _rows_of(_tensor(out, "out", device), "out")
+    if residual is not None:
+        _tensor(residual, "residual", device)
+        if residual.dtype is not out.dtype or tuple(residual.shape) != (*lead, n):
+            _fail("residual has not the result's type and shape")
+        if residual.dim() != 2:
+            try:
+                residual = residual.view(-1, n) if residual.numel() else residual.reshape(m, n)
+            except RuntimeError:
+                _fail("the leading axes of residual cannot be taken as one axis of rows: make it contiguous")
+        if n > 1 and m and residual.stride(1) != 1:
+            _fail("residual's last axis is not contiguous")
+    return out, y, _epilogue(n, device, bias, activation, residual)
+
+
+def matmul(x: Matrix, w: Matrix, bias=None, activation="linear", residual=None, dtype=torch.float32, out=None):
+    """activation(x w^T + bias) + residual, [x.rows, w.rows]."""
+    device = _matrix(x, "x").codes.device
+    _matrix(w, "w", device)
+    out, y, e = _linear_args((x.rows,), x.rows, w, device, bias, activation, residual, dtype, out)
+    check(lib.yl_mx_matmul(*_at(device), _ref(x._c), _ref(w._c), _ref(e) if e is not None else None, _ref(y)), "yl_mx_matmul")
+    return out
+
+
+def linear(x, w: Matrix, bias=None, activation="linear", residual=None, dtype=None, out=None):
+    """matmul(quantize(x), w, ...) on x [..., k], the same bits; the result has x's leading axes and, unless `dtype` says otherwise,
+    its type."""
+    device = _tensor(x, "x").device
+    _matrix(w, "w", device)
+    xd = _rows_of(x, "x")
+    m = xd.rows
+    out, y, e = _linear_args(tuple(x.shape[:-1]), m, w, device, bias, activation, residual, dtype or x.dtype, out)
+    need = lib.yl_mx_linear_workspace(m, xd.k)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(lib.yl_mx_linear(*_at(device), _ref(xd), _ref(w._c), _ref(e) if e is not None else None, _ref(y),
+                           ws.data_ptr() if need else None, need), "yl_mx_linear")
+    return out
+
+
+def conv2d(x: Matrix, filters: Matrix, batch: int, h: int, w: int, size: int, stride: int = 1, pad: int = 0, bias=None,
+           activation="linear", residual=None, out=None, want: str = "float"):
+    """The convolution of a quantised map with quantised filters.  `want`: "float" -> FP32 [batch, filters, oh, ow]; "mx" -> the next
+    layer's Matrix of batch * oh * ow rows; "both" -> the pair."""
+    device = _matrix(x, "x").codes.device
+    _matrix(filters, "filters", device)
+    if want not in ("float", "mx", "both"):
+        _fail("want is \"float\", \"mx\" or \"both\"")
+    if size < 1 or stride < 1 or pad < 0 or h + 2 * pad < size or w + 2 * pad < size:
+        _fail("the filter is larger than the padded map, or size, stride or pad is not one")
+    n, oh, ow = filters.rows, (h + 2 * pad - size) // stride + 1, (w + 2 * pad - size) // stride + 1
+    if residual is not None:
+        _tensor(residual, "residual", device)
+        if residual.dtype is not torch.float32 or tuple(residual.shape) != (batch, n, oh, ow) or not residual.is_contiguous():
+            _fail("residual is a contiguous float32 tensor of the result's shape")
+    if want == "mx":
+        if out is not None:
+            _fail("out is given, but want is \"mx\"")
+    elif out is None:
+        out = torch.empty(batch, n, oh, ow, dtype=torch.float32, device=device)
+    elif _tensor(out, "out", device).dtype is not torch.float32 or tuple(out.shape) != (batch, n, oh, ow) or not out.is_contiguous():
+        _fail("out is a contiguous float32 tensor of the result's shape")
+    q = Matrix.empty(batch * oh * ow, n, device) if want != "float" else None
+    e = _epilogue(n, device, bias, activation, residual)
+    shape = MxConv(batch, h, w, size, stride, pad)
+    check(lib.yl_mx_conv2d(*_at(device), _ref(x._c), _ref(filters._c), _ref(shape), _ref(e) if e is not None else None,
+                           out.data_ptr() if out is not None else None, _ref(q._c) if q is not None else None), "yl_mx_conv2d")
+    return q if want == "mx" else (out, q) if want == "both" else out
