@@ -182,6 +182,27 @@ def test_products(mx, m, n, k):
             close(mx.matmul(x, w, dtype=TYPES[dtype]), want, tol)
 
 
+def gpu_values(mx, q):
+    """The values of a matrix of finite blocks, float64 on the GPU (dequantize is compared with the oracle above)."""
+    return mx.dequantize(q).double()
+
+
+@pytest.mark.parametrize("m, n, k", [(1024, 1024, 96), (2000, 2050, 300), (4100, 4099, 130), (4096, 4096, 512), (257, 33_000, 64), (20_000, 900, 33), (1500, 260, 2100)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_products_that_fill_the_chip(mx, m, n, k, dtype):
+    """The same tolerance as mx_oracle.product_tolerance, computed on the GPU."""
+    x, w = mx.quantize(rand(m, k, seed=m, spread=0.5).cuda()), mx.quantize(rand(n, k, seed=n, spread=0.5).cuda())
+    res, b = rand(m, n, seed=3, dtype=dtype).cuda(), rand(n, seed=4).cuda()
+    y = mx.matmul(x, w, bias=b, activation="leaky", residual=res, dtype=TYPES[dtype]).double()
+    xv, wv = gpu_values(mx, x), gpu_values(mx, w)
+    v = xv @ wv.t() + b.double()
+    want = torch.where(v > 0, v, 0.1 * v) + res.double()
+    tol = ((o.blocks(k) + 1) // 2 + 16) * 2.0 ** -23 * (xv.abs() @ wv.abs().t())
+    tol = tol + 2.0 ** -22 * (v.abs() + want.abs() + tol) + 2.0 ** -24
+    tol = tol + o.HALF_STEP[dtype][0] * (want.abs() + tol)
+    assert ((y - want).abs() <= tol).all(), ((y - want).abs() - tol).max()
+
+
 @pytest.mark.parametrize("m, n, k", [(1, 100, 200), (7, 33, 64), (40, 129, 300), (130, 260, 96), (300, 300, 300)])
 @pytest.mark.parametrize("act", ["leaky", "relu", "logistic", "tanh", "elu", "relie", "ramp", "hardtan", "lhtan", "plse", "loggy"])
 def test_epilogues(mx, m, n, k, act):
@@ -323,6 +344,28 @@ def test_convolutions(mx, batch, c, n, h, w, size, stride, pad):
     r2 = res.cuda()
     z = mx.conv2d(q, fq, batch, h, w, size, stride, pad, bias=bias.cuda(), activation="leaky", residual=r2, out=r2)      # in place
     assert torch.equal(z, y)
+
+
+@pytest.mark.parametrize("batch, c, n, h, w, size, stride, pad", [(8, 32, 300, 50, 51, 3, 1, 1), (4, 160, 512, 61, 40, 3, 1, 1), (16, 128, 256, 64, 70, 3, 2, 1),
+                                                                  (30, 96, 513, 26, 26, 1, 1, 0), (3, 256, 2000, 70, 60, 1, 1, 0)])
+def test_convolutions_that_fill_the_chip(mx, batch, c, n, h, w, size, stride, pad):
+    x, f, *_ = conv_case(mx, 1, c, n, h, w, size, seed=c)
+    x = torch.cat([x * s for s in torch.linspace(0.5, 1.5, batch).tolist()])
+    q, fq = mx.quantize_nchw(x), mx.quantize_filters(f)
+    y, side = mx.conv2d(q, fq, batch, h, w, size, stride, pad, activation="leaky", want="both")
+    xv = gpu_values(mx, q).view(batch, h, w, c).permute(0, 3, 1, 2)
+    fv = gpu_values(mx, fq).view(n, size, size, -1)[..., :c].permute(0, 3, 1, 2)
+    xv, fv = xv.cpu(), fv.cpu()
+    some = [0, batch // 2, batch - 1]                             # the sums of three images on the CPU
+    v = torch.nn.functional.conv2d(xv[some], fv, stride=stride, padding=pad)
+    absum = torch.nn.functional.conv2d(xv[some].abs(), fv.abs(), stride=stride, padding=pad)
+    want = torch.where(v > 0, v, 0.1 * v)
+    tol = ((o.blocks(c) * size * size + 1) // 2 + 16) * 2.0 ** -23 * absum + 2.0 ** -22 * want.abs() + 2.0 ** -24
+    off = (y[some].cpu().double() - want).abs() - tol
+    assert (off <= 0).all(), off.max()
+    again = mx.quantize_nchw(y)
+    kb = o.blocks(n)
+    assert torch.equal(side.codes[:, :kb * 16], again.codes[:, :kb * 16]) and torch.equal(side.scales[:, :kb], again.scales[:, :kb])
 
 
 def test_a_convolution_of_size_one_is_the_product(mx):

@@ -10,7 +10,7 @@ namespace yl {
 namespace {
 
 constexpr int64_t MX_MAX_ELEMENTS = (int64_t)1 << 46;     // what a stride or a size may address: products of two stay in 64 bits
-constexpr int64_t MX_MAX_LD = (int64_t)1 << 20;           // blocks a row: 32-bit offsets inside a tile of rows
+constexpr int64_t MX_MAX_LD = (int64_t)1 << 19;           // blocks a row: 32-bit offsets inside a tile of 256 rows
 
 int refuse(const char *entry, const std::string &what)
 {
@@ -64,7 +64,7 @@ const char *check_matrix(const yl_mx_matrix *m)
 {
     if (!m) return "matrix is NULL";
     if (m->rows < 0 || m->k < 0) return "negative size of a matrix";
-    if (m->ld < blocks_of(m->k) || m->ld > MX_MAX_LD) return "ld of a matrix is smaller than its blocks, or above 2^20";
+    if (m->ld < blocks_of(m->k) || m->ld > MX_MAX_LD) return "ld of a matrix is smaller than its blocks, or above 2^19";
     if (m->rows > MX_MAX_ELEMENTS / (m->ld > 0 ? m->ld : 1)) return "matrix is too large";
     if (m->rows == 0 || m->k == 0) return nullptr;
     if (!m->codes || !m->scales) return "codes or scales of a matrix are NULL";
@@ -264,6 +264,10 @@ int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
     const int oh = oh_num / c.stride + 1, ow = ow_num / c.stride + 1;
     const int64_t J = (int64_t)c.batch * oh * ow, I = filters->rows;
     if (J > 0x7fffffff || I > 0x7fffffff || x->rows > 0x7fffffff || (J > 0 && I > MX_MAX_ELEMENTS / J)) return refuse(entry, "map or result is too large");
+    // the kernels' 32-bit offsets: the rows of the map under 256 neighbouring positions of the result
+    const int64_t area = (int64_t)oh * ow, part = 256 % area;
+    const int64_t reach = (256 / area + 1) * c.h * c.w + ((part + ow - 1) / ow + 1) * c.stride * c.w + (int64_t)(c.size + 1) * (c.w + 1);
+    if ((reach < x->rows ? reach : x->rows) + (int64_t)(c.size + 1) * (c.w + 1) > 0xFFFFFFFFLL / 16 / x->ld) return refuse(entry, "rows of the map are too far apart");
     const float *bias = epilogue ? epilogue->bias : nullptr;
     const float *residual = epilogue ? (const float *)epilogue->residual : nullptr;
     if ((uintptr_t)out % 4 || (uintptr_t)residual % 4) return refuse(entry, "out or residual is not aligned to its type");

@@ -13,7 +13,8 @@ typedef int mx_v8i __attribute__((ext_vector_type(8)));
 typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
 typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx_bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 mx_f16x4 __attribute__((ext_vector_type(4)));
 
 // one value of an ordinary tensor <-> FP32.  To FP16 / BF16: nearest even, half a step (2^-11 / 2^-8 of the value) at most.
 template <int TYPE>
@@ -29,6 +30,37 @@ __device__ __forceinline__ void mx_store(void *p, int64_t i, float v)
     if constexpr (TYPE == YL_F32) reinterpret_cast<float *>(p)[i] = v;
     else if constexpr (TYPE == YL_F16) reinterpret_cast<_Float16 *>(p)[i] = (_Float16)v;
     else reinterpret_cast<__bf16 *>(p)[i] = (__bf16)v;
+}
+
+// four neighbouring values, the first on a whole vector
+template <int TYPE>
+__device__ __forceinline__ void mx_store4(void *p, int64_t i, const float *v)
+{
+    if constexpr (TYPE == YL_F32) *reinterpret_cast<mx_f32x4 *>(reinterpret_cast<float *>(p) + i) = mx_f32x4{v[0], v[1], v[2], v[3]};
+    else if constexpr (TYPE == YL_F16) *reinterpret_cast<mx_f16x4 *>(reinterpret_cast<_Float16 *>(p) + i) = mx_f16x4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    else *reinterpret_cast<mx_bf16x4 *>(reinterpret_cast<__bf16 *>(p) + i) = mx_bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+}
+template <int TYPE>
+__device__ __forceinline__ void mx_load4(const void *p, int64_t i, float *v)
+{
+    if constexpr (TYPE == YL_F32) {
+        const mx_f32x4 x = *reinterpret_cast<const mx_f32x4 *>(reinterpret_cast<const float *>(p) + i);
+        for (int q = 0; q < 4; ++q) v[q] = x[q];
+    } else if constexpr (TYPE == YL_F16) {
+        const mx_f16x4 x = *reinterpret_cast<const mx_f16x4 *>(reinterpret_cast<const _Float16 *>(p) + i);
+        for (int q = 0; q < 4; ++q) v[q] = (float)x[q];
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned short *>(p) + i);
+        v[0] = __builtin_bit_cast(float, x.x << 16); v[1] = __builtin_bit_cast(float, x.x & 0xffff0000u);
+        v[2] = __builtin_bit_cast(float, x.y << 16); v[3] = __builtin_bit_cast(float, x.y & 0xffff0000u);
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void mx_add4(const void *p, int64_t i, float *v)
+{
+    float r[4];
+    mx_load4<TYPE>(p, i, r);
+    for (int q = 0; q < 4; ++q) v[q] += r[q];
 }
 
 // The scale byte of a block whose largest magnitude has the FP32 bits `top` (exponent field f): floor(log2) is f - 127, the largest
