@@ -167,7 +167,7 @@ int yl_network_batch(const yl_network *net);
 /* dims[3] = {w, h, c} of the network input */
 int yl_network_input_dims(const yl_network *net, int *dims);
 /* info[24]: type, batch, w, h, c, n, size, stride, pad, out_w, out_h, out_c,
- *           outputs, inputs, activation, xnor, quantized(int8 used), index,
+ *           outputs, inputs, activation, xnor, quantized (1 int8, 2 bf16, 3 mxfp4), index,
  *           classes, coords, total, softmax, reserved, batch_normalize */
 int yl_network_layer_info(const yl_network *net, int i, int *info);
 /* YOLO/REGION layer i: mask[n] (yolo: l.mask; region: 0..n-1) and anchors[2*total] (l.biases);
@@ -346,6 +346,12 @@ int yl_network_set_variant(yl_network *net, int bits);
  * tests/test_gpu_parity.py::test_fp32_error_vs_float64_truth) at ~0.55x the throughput (bench_detail.json
  * "strict_fp32"). */
 #define YL_PRECISION_FP32_STRICT 2
+/* Opt-in MXFP4 variant of the FP32 path (BEFORE yl_network_to_device): the convolutions that `quantized` would run in INT8 under
+ * YL_QUANT_RULE_CPU (not the first layer, not linear heads) and whose input has whole blocks of 32 channels run as yl_mx_conv2d:
+ * input and weights rounded to MXFP4 (yl_mx_quantize's rule, no calibration), FP32 accumulation, bias, activation and fused
+ * [shortcut]; with yl_network_set_fusion the rounded input of a layer is written by the convolution in front of it.  Rounding to
+ * 4 bits is far outside the FP32 path's contract: a network has to be trained or tuned for it. */
+#define YL_PRECISION_MXFP4 3
 int yl_network_set_precision(yl_network *net, int precision);
 /* the same for the INT8 convolution (conv_i8_mfma.hip): 0 = heuristic, 1 = 64x128, 2 = 32x256, 3 = 128x128,
  * 4 = 128x256 (8 waves), 5 = 64x256, 6 / 7 = 128x128 / 64x128 with half-depth LDS panels */

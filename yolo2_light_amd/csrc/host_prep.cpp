@@ -166,6 +166,10 @@ void select_conv_modes(Network &net) {
         else if (l.xnor && l.stride == 1 && l.pad == 1 && l.size == 3) l.conv_mode = CONV_XNOR;
         // opt-in (yl_network_set_precision): FP32 convolutions with whole 8-channel groups take bf16 operands
         else if (net.precision == YL_PRECISION_BF16 && !l.xnor && (l.c % 8) == 0 && l.size <= 5) l.conv_mode = CONV_BF16;
+        // opt-in: MXFP4 operands for the convolutions that the CPU rule above would run in INT8 (not the first, not linear heads), where
+        // whole blocks of 32 channels come in
+        else if (net.precision == YL_PRECISION_MXFP4 && !l.xnor && i >= 1 && l.activation != YL_LINEAR && (l.c % 32) == 0 && l.size <= 5 &&
+                 l.pad >= 0 && l.pad < l.size) l.conv_mode = CONV_MX4;
         else l.conv_mode = CONV_F32;
     }
 }

@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "mx.h"
 #include "yl_internal.h"
 #include "../../include/yolo2_hip_lab.h"
 
@@ -381,6 +382,22 @@ static int upload_conv(Network &net, Layer &l)
         }
         const size_t qb = (size_t)net.batch * l.h * l.w * l.Cpad * 2;
         if (qb > net.qbuf_bytes) net.qbuf_bytes = qb;
+    } else if (l.conv_mode == CONV_MX4) {
+        // one row a filter, tap after tap, the channels of a tap in blocks of 32 (yl_mx_conv2d's filters), rounded on the device
+        const int G = l.c / MX_BLOCK;
+        l.Cpad = l.c;
+        l.mx_ld = yl_mx_blocks((int64_t)taps * l.c);
+        const size_t codes = (size_t)M * l.mx_ld * 16, bytes = codes + (size_t)M * l.mx_ld;
+        YL_HIP(hipMalloc((void **)&l.d_weights_i8, bytes));
+        l.packed_bytes[2] = bytes;
+        int rc = pack_source_to_device(net, l.weights.data(), sizeof(float) * (size_t)M * K, nullptr, M);
+        if (rc != YL_OK) return rc;
+        for (int t = 0; t < taps; ++t) {
+            const MxDense src{reinterpret_cast<const float *>(net.d_pack_src) + t, YL_F32, 1, M, l.c, 0, (int64_t)l.c * taps, taps};
+            YL_LAUNCH(launch_mx_quantize(src, l.d_weights_i8 + (size_t)t * G * 16, l.d_weights_i8 + codes + (size_t)t * G, l.mx_ld, s), "mx_quantize_filters");
+        }
+        const size_t qb = (size_t)net.batch * l.h * l.w * G * 17;
+        if (qb > net.qbuf_bytes) net.qbuf_bytes = qb;
     } else {   // CONV_XNOR
         if (!l.xnor_ready) { set_error("XNOR layer without yl_network_calculate_binary_weights()"); return YL_ERR_STATE; }
         // 64-bit sign words along channels, filter pairs interleaved: [Mpad/2][Cw][2][9]; bit = (w > 0) (src/additionally.c:123,1544);
@@ -426,7 +443,7 @@ static int upload_conv(Network &net, Layer &l)
         if (ob > bb) bb = ob;
         if (bb > net.bitbuf_bytes) net.bitbuf_bytes = bb;
     }
-    if (net.debug && l.conv_mode != CONV_F32 && l.conv_mode != CONV_BF16) {
+    if (net.debug && l.conv_mode != CONV_F32 && l.conv_mode != CONV_BF16 && l.conv_mode != CONV_MX4) {
         YL_HIP(hipMalloc((void **)&l.d_debug, sizeof(int32_t) * (size_t)net.batch * l.outputs));
     }
     return YL_OK;
@@ -549,6 +566,7 @@ static int to_device(Network &net, int device)
     }
     // three quantised-activation buffers used round-robin (layer j reads ring[j % 3]): a producer
     // one or two layers earlier can write layer j's input while reading its own
+    net.qbuf_bytes = (net.qbuf_bytes + 255) & ~(size_t)255;
     if (net.qbuf_bytes) YL_HIP(hipMalloc((void **)&net.d_qbuf, 3 * net.qbuf_bytes));
     if (net.bitbuf_bytes) {
         net.bitbuf_bytes = (net.bitbuf_bytes + 255) & ~(size_t)255;
@@ -643,6 +661,8 @@ static int to_device(Network &net, int device)
         o.force_tile = 0;
         cv.pool_follows = conv_f32_pool_fusable(a, o);
     }
+    // channels in a 16-byte unit of a convolution's rounded input (0: it has none)
+    auto units_in = [](const Layer &l) { return l.conv_mode == CONV_INT8 ? 16 : l.conv_mode == CONV_BF16 ? 8 : l.conv_mode == CONV_MX4 ? MX_BLOCK : 0; };
     if (net.fuse && !net.debug) {
         const int nl = (int)net.layers.size();
         auto referenced_elsewhere = [&](int t, int consumer) {
@@ -659,8 +679,8 @@ static int to_device(Network &net, int device)
         };
         for (int j = 1; j < nl; ++j) {
             Layer &cons = net.layers[j];
-            if (cons.type != YL_CONVOLUTIONAL || !(cons.conv_mode == CONV_INT8 || cons.conv_mode == CONV_BF16)) continue;
-            const int uc = cons.conv_mode == CONV_BF16 ? 8 : 16;            // channels per 16-byte unit
+            if (cons.type != YL_CONVOLUTIONAL || !units_in(cons)) continue;
+            const int uc = units_in(cons);            // channels per 16-byte unit
             // the tensor layer j consumes is the output of layer j-1
             int prod = j - 1;                                  // layer whose kernel writes that tensor
             const Layer &in_l = net.layers[j - 1];
@@ -685,8 +705,8 @@ static int to_device(Network &net, int device)
         for (int j = 1; j < nl; ++j) {
             Layer &cons = net.layers[j];
             Layer &rt = net.layers[j - 1];
-            if (cons.type != YL_CONVOLUTIONAL || !(cons.conv_mode == CONV_INT8 || cons.conv_mode == CONV_BF16) || cons.q_from_producer) continue;
-            const int uc = cons.conv_mode == CONV_BF16 ? 8 : 16;
+            if (cons.type != YL_CONVOLUTIONAL || !units_in(cons) || cons.q_from_producer) continue;
+            const int uc = units_in(cons);
             if (rt.type != YL_ROUTE || rt.d_output_alias || rt.n < 2 || referenced_elsewhere(j - 1, j)) continue;
             // channel groups beyond c (Cpad rounds the group count up to a power of two) are never written on this
             // path: harmless for int8 (anything x zero weights = 0), not for bf16 (stale NaN / Inf x 0 = NaN)
@@ -1020,6 +1040,45 @@ static int forward_layer(Network &net, size_t i, const float *input)
             a.B = B; a.Cpad = l.Cpad; a.H = l.h; a.W = l.w; a.M = l.n; a.Mpad = l.Mpad; a.OH = l.out_h; a.OW = l.out_w;
             a.size = l.size; a.stride = l.stride; a.pad = l.pad; a.act = kernel_act;
             YL_LAUNCH(launch_conv_bf16(a, net.i8_tile, s, l.kernel_name, sizeof(l.kernel_name)), "conv_bf16");
+        } else if (l.conv_mode == CONV_MX4) {
+            // a ring slot holds the codes of the whole batch's map, then its scales
+            auto slot = [&](int layer) { return net.d_qbuf + (layer % 3) * net.qbuf_bytes; };
+            const int G = l.c / MX_BLOCK, HW = l.h * l.w;
+            int8_t *codes = slot((int)i), *scales = codes + (size_t)B * HW * G * 16;
+            auto round_map = [&](const float *from, int c, int g) {
+                const MxDense src{from, YL_F32, B, HW, c, (int64_t)c * HW, 1, HW};
+                return launch_mx_quantize(src, codes + (size_t)g * 16, scales + g, G, s);
+            };
+            if (l.q_from_route) {
+                const Layer &rt = net.layers[i - 1];
+                int g_off = 0;
+                for (int k = 0; k < rt.n; ++k) {
+                    const Layer &src = net.layers[rt.input_layers[k]];
+                    YL_LAUNCH(round_map(src.d_output, src.out_c, g_off), "mx_quantize_route");
+                    g_off += src.out_c / MX_BLOCK;
+                }
+            } else if (!l.q_from_producer)
+                YL_LAUNCH(round_map(input, l.c, 0), "mx_quantize");
+            MxProductArgs a;
+            a.a_codes = l.d_weights_i8; a.a_scales = l.d_weights_i8 + (size_t)l.n * l.mx_ld * 16; a.a_ld = l.mx_ld;
+            a.b_codes = codes; a.b_scales = scales; a.b_ld = G;
+            a.I = l.n; a.J = (int64_t)B * l.out_h * l.out_w; a.kb = (int64_t)l.size * l.size * G;
+            a.bias = l.d_biases; a.act = kernel_act; a.type = YL_F32; a.residual = nullptr; a.residual_stride = 0; a.out_stride = 0;
+            a.out = l.skip_f32_out ? nullptr : l.d_output;
+            if (l.fused_shortcut >= 0) {
+                Layer &sc = net.layers[l.fused_shortcut];
+                a.residual = net.layers[sc.index].d_output;
+                a.out = sc.d_output;
+            }
+            if (l.q_out_layer >= 0) {
+                const Layer &nx = net.layers[l.q_out_layer];
+                a.q_ld = nx.c / MX_BLOCK;
+                a.q_codes = slot(l.q_out_layer);
+                a.q_scales = slot(l.q_out_layer) + (size_t)a.J * a.q_ld * 16;
+            }
+            a.conv = true;
+            a.H = l.h; a.W = l.w; a.OH = l.out_h; a.OW = l.out_w; a.G = G; a.size = l.size; a.stride = l.stride; a.pad = l.pad; a.batch = B;
+            YL_LAUNCH(launch_mx_product(a, s, l.kernel_name, sizeof(l.kernel_name)), "mx_product");
         } else {
             auto ring = [&](int slot) { return net.d_bitbuf + (size_t)(slot % 3) * (net.bitbuf_bytes / sizeof(uint64_t)); };
             uint64_t *in_bits = ring((int)i);
@@ -1421,7 +1480,7 @@ int yl_network_layer_info(const yl_network *net, int i, int *info)
     info[0] = l.type; info[1] = l.batch; info[2] = l.w; info[3] = l.h; info[4] = l.c; info[5] = l.n;
     info[6] = l.size; info[7] = l.stride; info[8] = l.pad; info[9] = l.out_w; info[10] = l.out_h;
     info[11] = l.out_c; info[12] = l.outputs; info[13] = l.inputs; info[14] = l.activation;
-    info[15] = l.xnor; info[16] = (l.type == YL_CONVOLUTIONAL && l.conv_mode == CONV_INT8) ? 1 : ((l.type == YL_CONVOLUTIONAL && l.conv_mode == CONV_BF16) ? 2 : 0);
+    info[15] = l.xnor; info[16] = (l.type == YL_CONVOLUTIONAL && l.conv_mode == CONV_INT8) ? 1 : ((l.type == YL_CONVOLUTIONAL && l.conv_mode == CONV_BF16) ? 2 : (l.type == YL_CONVOLUTIONAL && l.conv_mode == CONV_MX4) ? 3 : 0);
     info[17] = l.index; info[18] = l.classes; info[19] = l.coords; info[20] = l.total;
     info[21] = l.softmax; info[22] = (l.type == YL_CONVOLUTIONAL) ? l.conv_mode : 0; info[23] = l.batch_normalize;
     return YL_OK;
@@ -1469,6 +1528,10 @@ int yl_network_layer_traffic(const yl_network *net, int i, double *bytes)
             const double h_in = 2.0 * B * (double)l.h * l.w * (l.Cpad ? l.Cpad : l.c);
             if (!l.q_from_producer) { rd += 4 * in_el; wr += h_in; }      // stand-alone pack pass
             rd += h_in + 2 * wel;
+        } else if (l.conv_mode == CONV_MX4) {
+            const double packed = 17.0 / 32.0, h_in = packed * in_el;     // a code and its share of the block's scale
+            if (!l.q_from_producer) { rd += 4 * in_el; wr += h_in; }      // stand-alone rounding pass
+            rd += h_in + packed * wel;
         } else if (l.conv_mode == CONV_XNOR) {
             const double bits = B * (double)l.h * l.w * 8.0 * ((l.c + 63) / 64);
             if (!l.bits_from_producer) { rd += 4 * in_el; wr += bits; }   // stand-alone sign-pack pass
@@ -1490,7 +1553,7 @@ int yl_network_layer_traffic(const yl_network *net, int i, double *bytes)
         if (fused) { rd += 4 * out_el; wr += 4 * out_el; }                // [shortcut] operand in, sum out
         else if (!l.skip_f32_out) wr += 4 * out_el;
         if (l.fused_pool >= 0) wr += out_el;                              // the pooled tensor of the fused [maxpool]: a quarter of the elements
-        if (l.q_out_layer >= 0) wr += (l.conv_mode == CONV_BF16 ? 2 : 1) * out_el;   // int8 / bf16 side output
+        if (l.q_out_layer >= 0) wr += (l.conv_mode == CONV_BF16 ? 2 : l.conv_mode == CONV_MX4 ? 17.0 / 32.0 : 1) * out_el;   // int8 / bf16 / MXFP4 side output
         break;
     }
     case YL_SHORTCUT:
@@ -1891,7 +1954,7 @@ int yl_network_set_variant(yl_network *net, int bits)
 
 int yl_network_set_precision(yl_network *net, int precision)
 {
-    if (!net || (precision != YL_PRECISION_FP32 && precision != YL_PRECISION_BF16 && precision != YL_PRECISION_FP32_STRICT)) {
+    if (!net || (precision != YL_PRECISION_FP32 && precision != YL_PRECISION_BF16 && precision != YL_PRECISION_FP32_STRICT && precision != YL_PRECISION_MXFP4)) {
         set_error("bad argument");
         return YL_ERR_ARG;
     }

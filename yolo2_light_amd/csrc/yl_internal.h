@@ -14,7 +14,7 @@
 namespace yl {
 
 // which convolution implementation a CONVOLUTIONAL layer runs with
-enum ConvMode { CONV_F32 = 0, CONV_INT8 = 1, CONV_XNOR = 2, CONV_BF16 = 3 };
+enum ConvMode { CONV_F32 = 0, CONV_INT8 = 1, CONV_XNOR = 2, CONV_BF16 = 3, CONV_MX4 = 4 };
 enum HostKind { HOST_NONE = 0, HOST_CALLER = 1, HOST_PINNED = 2 };
 
 constexpr int PREDICT_MAX_SPLIT = 4;  // sub-batches of one yl_network_predict call
@@ -69,8 +69,10 @@ struct Layer {
     void *d_weights_r3 = nullptr;        // FP32 3x3/1/1, C % 16 == 0: the row-transformed weights as three bf16 pieces (conv_f32_row3.hip), else nullptr
     unsigned *d_tile_ctr = nullptr;      //       8 work counters (one per XCD) of the persistent Winograd form, zero between launches
     size_t packed_bytes[6] = {0, 0, 0, 0, 0, 0};   // bytes of d_weights_t, d_wino32_u, d_weights_i8, d_weights_bits, d_weights_x3, d_weights_r3 (yl_debug_layer_packed)
-    int8_t *d_weights_i8 = nullptr;      // INT8: [K16pad][Mpad][16] int8 units; BF16: [K8pad][Mpad][8] bf16 units
-    int   Cpad = 0;                      // channels of the 16-byte-unit activation tensor (INT8: 16 per unit, BF16: 8)
+    int8_t *d_weights_i8 = nullptr;      // INT8: [K16pad][Mpad][16] int8 units; BF16: [K8pad][Mpad][8] bf16 units;
+                                         // MXFP4: codes [n][mx_ld][16], then scales [n][mx_ld]
+    int64_t mx_ld = 0;                   // MXFP4: row stride of the filters in blocks of 32 (taps * c / 32, rounded up to 4)
+    int   Cpad = 0;                      // channels of the 16-byte-unit activation tensor (INT8: 16 per unit, BF16: 8, MXFP4: 32)
     float bias_abs_max = 0.f;            // INT8: max |bias| and the smallest non-zero |bias| (-1 = a bias is not finite):
     float bias_abs_min_nz = 0.f;         //       the host's proof that the exact epilogue's corners cannot occur
     uint64_t *d_weights_bits = nullptr;  // XNOR: [Mpad][taps][Cw] 64-bit words

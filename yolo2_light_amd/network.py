@@ -65,7 +65,7 @@ class Network:
              device: Optional[int] = None, debug: bool = False, fuse: bool = False,
              quant_rule: int = 0, winograd: bool = True, bf16: bool = False, device_prep: bool = False,
              variant: Optional[int] = None, device_pack: Optional[bool] = None, strict: bool = False,
-             split_k: bool = False) -> "Network":
+             split_k: bool = False, mxfp4: bool = False) -> "Network":
         """The full prep sequence of test_detector_cpu (src/main.c:160-171)."""
         net = cls.from_cfg(cfg_path, batch, quantized)
         if quant_rule:
@@ -76,6 +76,8 @@ class Network:
             net.set_precision(1)
         if strict:
             net.set_precision(2)
+        if mxfp4:
+            net.set_precision(3)
         if split_k:
             check(lib.yl_network_set_split_k(net._h, 1), "yl_network_set_split_k")
         if variant is not None:
@@ -214,7 +216,7 @@ class Network:
 
     def set_precision(self, precision: int) -> None:
         """0 = FP32 (default), 1 = opt-in BF16 operands for the FP32 convolutions, 2 = strict FP32 (FP32-MFMA direct kernels
-        only); before to_device"""
+        only), 3 = opt-in MXFP4 operands for the convolutions that the INT8 rule covers; before to_device"""
         check(lib.yl_network_set_precision(self._h, precision), "yl_network_set_precision")
 
     def set_variant(self, bits: int) -> None:
