@@ -268,6 +268,8 @@ int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
     const int64_t area = (int64_t)oh * ow, part = 256 % area;
     const int64_t reach = (256 / area + 1) * c.h * c.w + ((part + ow - 1) / ow + 1) * c.stride * c.w + (int64_t)(c.size + 1) * (c.w + 1);
     if ((reach < x->rows ? reach : x->rows) + (int64_t)(c.size + 1) * (c.w + 1) > 0xFFFFFFFFLL / 16 / x->ld) return refuse(entry, "rows of the map are too far apart");
+    if (x->k > 1 << 18) return refuse(entry, "more than 2^18 channels");
+    if ((256 / area + 2) > 0xFFFFFFFFLL / 4 / (area * (I > 0 ? I : 1))) return refuse(entry, "an image's result is too large");
     const float *bias = epilogue ? epilogue->bias : nullptr;
     const float *residual = epilogue ? (const float *)epilogue->residual : nullptr;
     if ((uintptr_t)out % 4 || (uintptr_t)residual % 4) return refuse(entry, "out or residual is not aligned to its type");

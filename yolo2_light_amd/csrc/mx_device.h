@@ -13,8 +13,8 @@ typedef int mx_v8i __attribute__((ext_vector_type(8)));
 typedef float mx_f32x2 __attribute__((ext_vector_type(2)));
 typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mx_f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 mx_bf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 mx_f16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 mx_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 mx_f16x8 __attribute__((ext_vector_type(8)));
 
 // one value of an ordinary tensor <-> FP32.  To FP16 / BF16: nearest even, half a step (2^-11 / 2^-8 of the value) at most.
 template <int TYPE>
@@ -32,36 +32,42 @@ __device__ __forceinline__ void mx_store(void *p, int64_t i, float v)
     else reinterpret_cast<__bf16 *>(p)[i] = (__bf16)v;
 }
 
-// four neighbouring values, the first on a whole vector
+// 16 bytes of neighbouring values, the first on a whole vector: 4 of FP32, 8 of the others
 template <int TYPE>
-__device__ __forceinline__ void mx_store4(void *p, int64_t i, const float *v)
+constexpr int MX_VEC = TYPE == YL_F32 ? 4 : 8;
+typedef unsigned mx_u32x4 __attribute__((ext_vector_type(4)));
+template <int TYPE>
+__device__ __forceinline__ mx_u32x4 mx_pack(const float *v)
 {
-    if constexpr (TYPE == YL_F32) *reinterpret_cast<mx_f32x4 *>(reinterpret_cast<float *>(p) + i) = mx_f32x4{v[0], v[1], v[2], v[3]};
-    else if constexpr (TYPE == YL_F16) *reinterpret_cast<mx_f16x4 *>(reinterpret_cast<_Float16 *>(p) + i) = mx_f16x4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-    else *reinterpret_cast<mx_bf16x4 *>(reinterpret_cast<__bf16 *>(p) + i) = mx_bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    if constexpr (TYPE == YL_F32) return __builtin_bit_cast(mx_u32x4, mx_f32x4{v[0], v[1], v[2], v[3]});
+    else if constexpr (TYPE == YL_F16) return __builtin_bit_cast(mx_u32x4, mx_f16x8{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3], (_Float16)v[4], (_Float16)v[5], (_Float16)v[6], (_Float16)v[7]});
+    else return __builtin_bit_cast(mx_u32x4, mx_bf16x8{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3], (__bf16)v[4], (__bf16)v[5], (__bf16)v[6], (__bf16)v[7]});
 }
 template <int TYPE>
-__device__ __forceinline__ void mx_load4(const void *p, int64_t i, float *v)
+__device__ __forceinline__ void mx_unpack(mx_u32x4 x, float *v)
 {
     if constexpr (TYPE == YL_F32) {
-        const mx_f32x4 x = *reinterpret_cast<const mx_f32x4 *>(reinterpret_cast<const float *>(p) + i);
-        for (int q = 0; q < 4; ++q) v[q] = x[q];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const unsigned w = x[q];                       // a copy: the cast of the element itself gives element 0
+            v[q] = __builtin_bit_cast(float, w);
+        }
     } else if constexpr (TYPE == YL_F16) {
-        const mx_f16x4 x = *reinterpret_cast<const mx_f16x4 *>(reinterpret_cast<const _Float16 *>(p) + i);
-        for (int q = 0; q < 4; ++q) v[q] = (float)x[q];
+        const mx_f16x8 h = __builtin_bit_cast(mx_f16x8, x);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = (float)h[q];
     } else {
-        const uint2 x = *reinterpret_cast<const uint2 *>(reinterpret_cast<const unsigned short *>(p) + i);
-        v[0] = __builtin_bit_cast(float, x.x << 16); v[1] = __builtin_bit_cast(float, x.x & 0xffff0000u);
-        v[2] = __builtin_bit_cast(float, x.y << 16); v[3] = __builtin_bit_cast(float, x.y & 0xffff0000u);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            v[2 * q] = __builtin_bit_cast(float, x[q] << 16);
+            v[2 * q + 1] = __builtin_bit_cast(float, x[q] & 0xffff0000u);
+        }
     }
 }
 template <int TYPE>
-__device__ __forceinline__ void mx_add4(const void *p, int64_t i, float *v)
-{
-    float r[4];
-    mx_load4<TYPE>(p, i, r);
-    for (int q = 0; q < 4; ++q) v[q] += r[q];
-}
+__device__ __forceinline__ mx_u32x4 mx_load_vec(const void *p, int64_t i) { return *reinterpret_cast<const mx_u32x4 *>(reinterpret_cast<const char *>(p) + i * (16 / MX_VEC<TYPE>)); }
+template <int TYPE>
+__device__ __forceinline__ void mx_store_vec(void *p, int64_t i, mx_u32x4 v) { *reinterpret_cast<mx_u32x4 *>(reinterpret_cast<char *>(p) + i * (16 / MX_VEC<TYPE>)) = v; }
 
 // The scale byte of a block whose largest magnitude has the FP32 bits `top` (exponent field f): floor(log2) is f - 127, the largest
 // E2M1 exponent is 2, so the byte is f - 2, not below 0 (2^-127; subnormals and zero have f = 0).  f = 255 is an Inf or a NaN.

@@ -32,94 +32,141 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_v4i a, mx_v4i b, mx_f32x16 c, in
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a), mx_operand(b), c, 4, 4, S, sa, S, sb);
 }
 
-// A strip of D, 32 rows from ib by COLS columns from jb, in LDS: + bias, activation, + residual, to rows of memory.  A lane takes four
-// neighbouring columns.
-template <int TYPE, int COLS, int PITCH>
+// LINEAR, LEAKY and RELU in line (activations.h's arithmetic); the others only where RARE says so
+template <bool RARE>
+__device__ __forceinline__ float mx_activate(float v, int act)
+{
+    if constexpr (RARE) return yl_act_epilogue(v, act);
+    else return v > 0.f || act == YL_LINEAR ? v : act == YL_LEAKY ? (float)(.1 * (double)v) : __fmul_rn(v, 0.f);
+}
+
+// A strip of D, 32 rows from ib by COLS columns from jb, in LDS: + bias, activation, + residual, to rows of memory.  In 16-byte vectors
+// where every row's begin on one, else by single values; AHEAD rows' addends are requested before the first is used.
+template <int TYPE, bool RARE, bool WIDE, int COLS, int PITCH>
 __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const float *strip, int ib, int jb, int lane)
 {
-    constexpr int LANES = COLS / 4, ROWS = 64 / LANES;     // lanes a row, rows a step
-    const int c = lane % LANES * 4, j = jb + c, J = (int)p.J;
-    const int rows = min(32, (int)p.I - ib);
-    const int n = min(4, J - j);
-    if (n <= 0) return;
-    constexpr int BYTES = TYPE == YL_F32 ? 4 : 2;
-    // four values at once where every row's begin on a whole vector
-    const bool wide = n == 4 && p.out_stride % 4 == 0 && (uintptr_t)p.out % (4 * BYTES) == 0 &&
-                      (!p.residual || (p.residual_stride % 4 == 0 && (uintptr_t)p.residual % (4 * BYTES) == 0));
-    float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias)
-        for (int q = 0; q < 4; ++q) bias[q] = q < n ? p.bias[j + q] : 0.f;
-    for (int r = lane / LANES; r < rows; r += ROWS) {
-        const mx_f32x4 s = *reinterpret_cast<const mx_f32x4 *>(strip + r * PITCH + c);
-        float v[4];
+    constexpr int VEC = WIDE ? MX_VEC<TYPE> : 1;
+    constexpr int LANES = COLS / VEC < 64 ? COLS / VEC : 64;   // lanes a row
+    constexpr int ROWS = 64 / LANES, STEPS = 32 / ROWS, AHEAD = STEPS < 4 ? STEPS : 4;
+    const int rows = min(32, (int)p.I - ib), act = p.act;
+    const int64_t out_step = (int64_t)p.out_stride * ROWS, res_step = (int64_t)p.residual_stride * ROWS;
+    const bool add = p.residual != nullptr;
+    for (int c = lane % LANES * VEC; c < COLS; c += LANES * VEC) {
+        const int j = jb + c;
+        if (j >= (int)p.J) return;
+        float bias[VEC];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = s[q] + bias[q];
-        if (p.act != YL_LINEAR) {
+        for (int q = 0; q < VEC; ++q) bias[q] = p.bias ? p.bias[j + q] : 0.f;
+        const int r0 = lane / LANES;
+        int64_t at = (int64_t)(ib + r0) * p.out_stride + j, res = (int64_t)(ib + r0) * p.residual_stride + j;
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q) {                  // one copy of the activations' code
-                const float y = yl_act_epilogue(q == 0 ? v[0] : q == 1 ? v[1] : q == 2 ? v[2] : v[3], p.act);
-                v[0] = q == 0 ? y : v[0]; v[1] = q == 1 ? y : v[1]; v[2] = q == 2 ? y : v[2]; v[3] = q == 3 ? y : v[3];
-            }
-        }
-        const int64_t at = (int64_t)(ib + r) * p.out_stride + j, res = (int64_t)(ib + r) * p.residual_stride + j;
-        if (wide) {
-            if (p.residual) mx_add4<TYPE>(p.residual, res, v);
-            mx_store4<TYPE>(p.out, at, v);
-        } else {
+        for (int step = 0; step < STEPS; step += AHEAD) {
+            float v[AHEAD][VEC];
+            mx_u32x4 rv[AHEAD];
+            float rs[AHEAD];
+            if (add) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (q < n) {
-                    if (p.residual) v[q] += mx_load<TYPE>(p.residual, res + q);
-                    mx_store<TYPE>(p.out, at + q, v[q]);
+                for (int s = 0; s < AHEAD; ++s) {
+                    const bool ok = r0 + (step + s) * ROWS < rows;
+                    if constexpr (WIDE) rv[s] = mx_load_vec<TYPE>(p.residual, ok ? res + s * res_step : res);
+                    else rs[s] = mx_load<TYPE>(p.residual, ok ? res + s * res_step : res);
                 }
+            }
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) {
+                const float *from = strip + (r0 + (step + s) * ROWS) * PITCH + c;
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int q = 0; q < VEC; q += 4) {
+                        const mx_f32x4 x = *reinterpret_cast<const mx_f32x4 *>(from + q);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[s][q + k] = x[k];
+                    }
+                } else v[s][0] = *from;
+            }
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) {
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) v[s][q] = mx_activate<RARE>(v[s][q] + bias[q], act);
+                if (add) {
+                    float r[8];
+                    if constexpr (WIDE) mx_unpack<TYPE>(rv[s], r);
+                    else r[0] = rs[s];
+#pragma unroll
+                    for (int q = 0; q < VEC; ++q) v[s][q] += r[q];
+                }
+                if (r0 + (step + s) * ROWS < rows) {
+                    if constexpr (WIDE) mx_store_vec<TYPE>(p.out, at + s * out_step, mx_pack<TYPE>(v[s]));
+                    else mx_store<TYPE>(p.out, at + s * out_step, v[s][0]);
+                }
+            }
+            at += AHEAD * out_step; res += AHEAD * res_step;
+            if (r0 + (step + AHEAD) * ROWS >= rows) break;
         }
     }
 }
 
-// The same for a convolution: rows are filters, columns positions; memory is planes of float, a lane takes a column.  With a side
-// output the strip's rows are one block of every column's result.
-template <int COLS, int PITCH>
-__device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, float *strip, int ib, int jb, int lane)
+// The 32 rows from ib of a position's result as one block of it.  y: this lane's 16 of them (rows 8 (e / 4) + 4 half + e % 4, zero where
+// there is none), the others are in lane l ^ 32.
+__device__ __forceinline__ void mx_side_block(const MxProductArgs &p, int64_t j, bool ok, int ib, int half, const float *y)
 {
-    const int rows = min(32, (int)p.I - ib), area = p.OH * p.OW;
-    for (int c = lane; c < COLS; c += 64) {
-        const int j = jb + c;
-        if (j >= (int)p.J) continue;
-        const int image = j / area;
-        int64_t at = ((int64_t)image * p.I + ib) * area + (j - image * area);
-        const float *residual = reinterpret_cast<const float *>(p.residual);
-        float *out = reinterpret_cast<float *>(p.out);
-        unsigned top = 0;
-#pragma unroll 4
-        for (int r = 0; r < rows; ++r, at += area) {
-            float v = strip[r * PITCH + c];
-            if (p.bias) v += p.bias[ib + r];
-            v = yl_act_epilogue(v, p.act);
-            if (residual) v += residual[at];
-            if (out) out[at] = v;
-            if (p.q_codes) strip[r * PITCH + c] = v;
-            top = max(top, mx_abs_bits(v));
-        }
-        if (!p.q_codes) continue;
-        const unsigned byte = mx_scale_byte(top);
-        unsigned w[4] = {0, 0, 0, 0};
-        if (byte != 255) {
+    unsigned top = 0;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                float v[8];
+    for (int e = 0; e < 16; ++e) top = max(top, mx_abs_bits(y[e]));
+    auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);      // {low half's, high half's} in every lane
+    const unsigned byte = mx_scale_byte(max(both[0], both[1]));
+    // four of a word's eight codes are this lane's: 16 bits each of the words 0-3
+    unsigned h0 = 0, h1 = 0;
+    if (byte != 255) { h0 = mx_codes8(y, byte); h1 = mx_codes8(y + 8, byte); }
+    auto w0 = __builtin_amdgcn_permlane32_swap(h0, h0, false, false);
+    auto w1 = __builtin_amdgcn_permlane32_swap(h1, h1, false, false);
+    if (!ok || half != 0) return;
+    const uint4 q = make_uint4((w0[0] & 0xffffu) | w0[1] << 16, w0[0] >> 16 | (w0[1] & 0xffff0000u),
+                               (w1[0] & 0xffffu) | w1[1] << 16, w1[0] >> 16 | (w1[1] & 0xffff0000u));
+    reinterpret_cast<uint4 *>(p.q_codes)[j * p.q_ld + ib / 32] = q;
+    reinterpret_cast<unsigned char *>(p.q_scales)[j * p.q_ld + ib / 32] = (unsigned char)byte;
+}
+
+// A convolution's 32 x 32 tile of D from registers to planes of memory.  `at`: byte offset of (this lane's position, row 0 of the image's
+// planes) in `out`, -1 where there is no such position.
+template <bool RARE>
+__device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const mx_f32x16 &acc, int ib, int64_t j, bool ok, int half,
+                                                 __amdgpu_buffer_rsrc_t out, __amdgpu_buffer_rsrc_t residual, int at)
+{
+    const int I = (int)p.I, plane = p.OH * p.OW * 4;
+    float y[16], add[16];
+    int off[16];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = 8 * g + q < rows ? strip[(8 * g + q) * PITCH + c] : 0.f;
-                w[g] = mx_codes8(v, byte);
-            }
-        }
-        reinterpret_cast<uint4 *>(p.q_codes)[j * p.q_ld + ib / 32] = make_uint4(w[0], w[1], w[2], w[3]);
-        reinterpret_cast<unsigned char *>(p.q_scales)[j * p.q_ld + ib / 32] = (unsigned char)byte;
+    for (int e = 0; e < 16; ++e) {
+        const int r = 8 * (e / 4) + e % 4;                 // + 4 half, in the lane's offset
+        off[e] = ok && ib + r + 4 * half < I ? at + 4 * half * plane : -1;
+        add[e] = 0.f;
+        if (p.residual) add[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(residual, off[e], (ib + r) * plane, 0));
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int i = ib + 8 * (e / 4) + e % 4 + 4 * half;
+        float v = acc[e];
+        if (p.bias) v += p.bias[min(i, I - 1)];
+        y[e] = mx_activate<RARE>(v, p.act);
+        if (p.residual) y[e] += add[e];
+    }
+    if (p.out) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y[e]), out, off[e], (ib + 8 * (e / 4) + e % 4) * plane, 0);
+    }
+    if (p.q_codes) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = off[e] != -1 ? y[e] : 0.f;
+        mx_side_block(p, j, ok, ib, half, y);
     }
 }
 
 struct MxTileDev {
     MxProductArgs p;
     int tiles_i, tiles_j;
+    unsigned g_magic;      // ceil(2^32 / G): block / G is the high half of the product while block * G < 2^32 (G = 1: 0)
 };
 
 // logical tile of a workgroup: every XCD (blockIdx % 8) gets one contiguous run of tiles, walked in bands of 8 tiles along i so that the
@@ -134,11 +181,11 @@ __device__ __forceinline__ void mx_tile_of(int bid, int nwg, int tiles_i, int ti
     ti = band * 8 + in - tj * high;
 }
 
-template <int TYPE, bool CONV, bool BYTES, int TI, int TJ>
-__global__ __launch_bounds__(MX_THREADS, TI * TJ > 4 ? 1 : 2) void mx_product_tile_kernel(MxTileDev d)
+template <int TYPE, bool CONV, bool BYTES, bool RARE, int TI, int TJ>
+__global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 2) void mx_product_tile_kernel(MxTileDev d)
 {
     constexpr int BI = 64 * TI, BJ = 64 * TJ;
-    constexpr int APT = BI / 32, BPT = BJ / 32, SPT = (BI + BJ) / 128;
+    constexpr int APT = BI / 32, BPT = BJ / 32, SPT = (BI + BJ + 127) / 128;
     constexpr int STAGE = (BI + BJ) * (MX_PANEL * 16 + MX_PANEL);
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
     const MxProductArgs &p = d.p;
@@ -199,15 +246,16 @@ __global__ __launch_bounds__(MX_THREADS, TI * TJ > 4 ? 1 : 2) void mx_product_ti
         const int row = tid / 2 + 128 * e;
         sout[e] = 0;
         if (row < BI) soff[e] = min(row, I - 1 - i0) * a_ld;
-        else soff[e] = (int)((unsigned)b_row(row - BI, sout[e]) * (unsigned)b_ld);
+        else soff[e] = (int)((unsigned)b_row(min(row - BI, BJ - 1), sout[e]) * (unsigned)b_ld);
     }
     const int code_at = (tid / 8) * 128 + ((unit ^ ((tid / 8) & 7)) * 16);
 
     // ---- a convolution's blocks in the order (tap, channel block): of this thread's unit, stepped by a panel at a time
+    auto tap_of = [&](int block) { return (int)__umulhi((unsigned)block, d.g_magic) + (p.G == 1 ? block : 0); };      // block / G
     int tap = 0, g = 0, step_tap = 0, step_g = 0;
     if (CONV) {
-        tap = unit / p.G; g = unit - tap * p.G;
-        step_tap = MX_PANEL / p.G; step_g = MX_PANEL - step_tap * p.G;
+        tap = tap_of(unit); g = unit - tap * p.G;
+        step_tap = tap_of(MX_PANEL); step_g = MX_PANEL - step_tap * p.G;
     }
     auto tap_row = [&](int t) {                        // tap -> rows of the map from the first tap
         const int ky = p.size == 3 ? (t * 11) >> 5 : (p.size == 1 ? 0 : t / p.size);
@@ -215,61 +263,56 @@ __global__ __launch_bounds__(MX_THREADS, TI * TJ > 4 ? 1 : 2) void mx_product_ti
     };
     auto outside_bit = [](unsigned m, int t) { return __builtin_amdgcn_sbfe((int)m, t, 1); };
 
+    // the panel's ITEMS requests and, in the same order, the stores of what they brought: one or two between two matrix instructions
+    constexpr int ITEMS = APT + BPT + SPT;
     mx_v4i areg[APT], breg[BPT];
     int sreg[SPT][BYTES ? 4 : 1];
-    auto load = [&](int pn) {                          // request panel pn (the panels in order, each once)
+    int here = 0, here_out[BPT];                       // conv: this thread's unit of the panel being requested, rows outside the image as -1
+    auto begin_load = [&](int pn) {                    // the panels in order, each once
         const int end = pn * MX_PANEL + unit >= kb ? -1 : 0;
-        const int at = pn * MX_PANEL * 16;
-#pragma unroll
-        for (int e = 0; e < APT; ++e) areg[e] = __builtin_bit_cast(mx_v4i, __builtin_amdgcn_raw_buffer_load_b128(ra, aoff[e] | end, at, 0));
+        here = end;
         if (CONV) {
-            const int here = tap_row(tap) * b_ld * 16 + g * 16;
+            here = tap_row(tap) * b_ld * 16 + g * 16;
 #pragma unroll
-            for (int e = 0; e < BPT; ++e)
-                breg[e] = __builtin_bit_cast(mx_v4i, __builtin_amdgcn_raw_buffer_load_b128(rb, (boff[e] + here) | outside_bit(bout[e], tap) | end, 0, 0));
+            for (int e = 0; e < BPT; ++e) here_out[e] = outside_bit(bout[e], tap) | end;
             tap += step_tap; g += step_g;
             if (g >= p.G) { g -= p.G; ++tap; }
-        } else {
-#pragma unroll
-            for (int e = 0; e < BPT; ++e) breg[e] = __builtin_bit_cast(mx_v4i, __builtin_amdgcn_raw_buffer_load_b128(rb, boff[e] | end, at, 0));
         }
-        const int block0 = pn * MX_PANEL + 4 * word;   // the word's first block
-#pragma unroll
-        for (int e = 0; e < SPT; ++e) {
+    };
+    auto load = [&](int pn, int k) {
+        const int at = pn * MX_PANEL * 16, end = pn * MX_PANEL + unit >= kb ? -1 : 0;
+        if (k < APT) areg[k] = __builtin_bit_cast(mx_v4i, __builtin_amdgcn_raw_buffer_load_b128(ra, aoff[k] | end, at, 0));
+        else if (k < APT + BPT) {
+            const int e = k - APT;
+            breg[e] = __builtin_bit_cast(mx_v4i, CONV ? __builtin_amdgcn_raw_buffer_load_b128(rb, (boff[e] + here) | here_out[e], 0, 0)
+                                                      : __builtin_amdgcn_raw_buffer_load_b128(rb, boff[e] | end, at, 0));
+        } else {
+            const int e = k - APT - BPT, block0 = pn * MX_PANEL + 4 * word;            // the word's first block
             const bool of_a = BI % 128 == 0 ? 128 * e < BI : tid / 2 + 128 * e < BI;
-            if constexpr (BYTES) {
+            // the word, or its bytes one by one
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int block = block0 + i, off_end = block >= kb ? -1 : 0;
-                    if (of_a) sreg[e][i] = __builtin_amdgcn_raw_buffer_load_b8(ras, (soff[e] + block) | off_end, 0, 0);
-                    else if (CONV) {
-                        const int t = block / p.G;
-                        sreg[e][i] = __builtin_amdgcn_raw_buffer_load_b8(rbs, (soff[e] + tap_row(t) * b_ld + block - t * p.G) | outside_bit(sout[e], min(t, 31)) | off_end, 0, 0);
-                    } else sreg[e][i] = __builtin_amdgcn_raw_buffer_load_b8(rbs, (soff[e] + block) | off_end, 0, 0);
+            for (int i = 0; i < (BYTES ? 4 : 1); ++i) {
+                const int block = block0 + i, off_end = block >= kb ? -1 : 0;
+                int off = (soff[e] + block) | off_end;
+                if (CONV && !of_a) {
+                    const int t = tap_of(block);
+                    off = (soff[e] + tap_row(t) * b_ld + block - t * p.G) | outside_bit(sout[e], min(t, 31)) | off_end;
                 }
-            } else {
-                const int off_end = block0 >= kb ? -1 : 0;
-                if (of_a) sreg[e][0] = __builtin_amdgcn_raw_buffer_load_b32(ras, (soff[e] + block0) | off_end, 0, 0);
-                else if (CONV) {
-                    const int t = block0 / p.G;
-                    sreg[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rbs, (soff[e] + tap_row(t) * b_ld + block0 - t * p.G) | outside_bit(sout[e], min(t, 31)) | off_end, 0, 0);
-                } else sreg[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rbs, (soff[e] + block0) | off_end, 0, 0);
+                if constexpr (BYTES) sreg[e][i] = of_a ? __builtin_amdgcn_raw_buffer_load_b8(ras, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b8(rbs, off, 0, 0);
+                else sreg[e][i] = of_a ? __builtin_amdgcn_raw_buffer_load_b32(ras, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(rbs, off, 0, 0);
             }
         }
     };
-    auto store = [&](int pn) {                         // panel pn: registers -> its half of LDS
+    auto store = [&](int pn, int k) {                  // registers -> the panel's half of LDS
         char *st = smem + (pn & 1) * STAGE;
-#pragma unroll
-        for (int e = 0; e < APT; ++e) *reinterpret_cast<mx_v4i *>(st + code_at + e * 4096) = areg[e];
-#pragma unroll
-        for (int e = 0; e < BPT; ++e) *reinterpret_cast<mx_v4i *>(st + BI * 128 + code_at + e * 4096) = breg[e];
-        const int left = kb - (pn * MX_PANEL + 4 * word);
-        const unsigned keep = left >= 4 ? 0xFFFFFFFFu : (left <= 0 ? 0u : (1u << (8 * left)) - 1u);     // scales behind the last block are not read
-#pragma unroll
-        for (int e = 0; e < SPT; ++e) {
+        if (k < APT) *reinterpret_cast<mx_v4i *>(st + code_at + k * 4096) = areg[k];
+        else if (k < APT + BPT) *reinterpret_cast<mx_v4i *>(st + BI * 128 + code_at + (k - APT) * 4096) = breg[k - APT];
+        else {
+            const int e = k - APT - BPT, left = kb - (pn * MX_PANEL + 4 * word);
+            const unsigned keep = left >= 4 ? 0xFFFFFFFFu : (left <= 0 ? 0u : (1u << (8 * left)) - 1u);     // scales behind the last block are not read
             unsigned w = (unsigned)sreg[e][0];
             if constexpr (BYTES) w = (w & 255u) | ((unsigned)sreg[e][1] & 255u) << 8 | ((unsigned)sreg[e][2] & 255u) << 16 | ((unsigned)sreg[e][3] & 255u) << 24;
-            *reinterpret_cast<unsigned *>(st + (BI + BJ) * 128 + (tid + 256 * e) * 4) = w & keep;
+            if ((BI + BJ) % 128 == 0 || tid + 256 * e < 2 * (BI + BJ)) *reinterpret_cast<unsigned *>(st + (BI + BJ) * 128 + (tid + 256 * e) * 4) = w & keep;
         }
     };
 
@@ -284,20 +327,17 @@ __global__ __launch_bounds__(MX_THREADS, TI * TJ > 4 ? 1 : 2) void mx_product_ti
     const int ar = (wi0 + l31) * 128, br = BI * 128 + (wj0 + l31) * 128, x7 = l31 & 7;
     mx_v4i af[2][TI], bf[2][TJ];
     int sa[TI], sb[TJ], sa_next[TI], sb_next[TJ];
-    auto fetch = [&](int pn, int s, int into) {        // operands of step s of panel pn
+    constexpr int READS = TI + TJ;
+    auto fetch = [&](int pn, int s, int into, int k) { // operands of step s of panel pn
         const char *st = smem + (pn & 1) * STAGE;
         const int at = ((4 * half + s) ^ x7) * 16;
-#pragma unroll
-        for (int i = 0; i < TI; ++i) af[into][i] = *reinterpret_cast<const mx_v4i *>(st + ar + at + i * 4096);
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) bf[into][j] = *reinterpret_cast<const mx_v4i *>(st + br + at + j * 4096);
+        if (k < TI) af[into][k] = *reinterpret_cast<const mx_v4i *>(st + ar + at + k * 4096);
+        else bf[into][k - TI] = *reinterpret_cast<const mx_v4i *>(st + br + at + (k - TI) * 4096);
     };
-    auto fetch_scales = [&](int pn) {
+    auto fetch_scale = [&](int pn, int k) {
         const char *st = smem + (pn & 1) * STAGE + (BI + BJ) * 128;
-#pragma unroll
-        for (int i = 0; i < TI; ++i) sa_next[i] = *reinterpret_cast<const int *>(st + (wi0 + i * 32 + l31) * 8 + half * 4);
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) sb_next[j] = *reinterpret_cast<const int *>(st + (BI + wj0 + j * 32 + l31) * 8 + half * 4);
+        if (k < TI) sa_next[k] = *reinterpret_cast<const int *>(st + (wi0 + k * 32 + l31) * 8 + half * 4);
+        else sb_next[k - TI] = *reinterpret_cast<const int *>(st + (BI + wj0 + (k - TI) * 32 + l31) * 8 + half * 4);
     };
     auto take_scales = [&]() {
 #pragma unroll
@@ -305,83 +345,122 @@ __global__ __launch_bounds__(MX_THREADS, TI * TJ > 4 ? 1 : 2) void mx_product_ti
 #pragma unroll
         for (int j = 0; j < TJ; ++j) sb[j] = sb_next[j];
     };
-#define MX_STEP(S, CUR)                                                                                                          \
-    _Pragma("unroll") for (int i = 0; i < TI; ++i)                                                                               \
-        _Pragma("unroll") for (int j = 0; j < TJ; ++j) acc[i][j] = mx_mfma<S>(af[CUR][i], bf[CUR][j], acc[i][j], sa[i], sb[j]);  \
-    __builtin_amdgcn_sched_barrier(0);
+    // step S of a panel: its matrix instructions, and between them the N calls of `other`, spread over the first WITHIN of them
+    auto spread = [](int m, int n, int within) { return m >= within ? n : m * n / within; };
+#define MX_STEP(S, CUR, N, WITHIN, OTHER)                                                                                        \
+    _Pragma("unroll") for (int m = 0; m < TI * TJ; ++m) {                                                                        \
+        acc[m / TJ][m % TJ] = mx_mfma<S>(af[CUR][m / TJ], bf[CUR][m % TJ], acc[m / TJ][m % TJ], sa[m / TJ], sb[m % TJ]);         \
+        _Pragma("unroll") for (int k = spread(m, N, WITHIN); k < spread(m + 1, N, WITHIN); ++k) { OTHER }                        \
+        __builtin_amdgcn_sched_barrier(0);                                                                                       \
+    }
 
     if (panels > 0) {
-        load(0);
-        store(0);
-        load(1);
+        begin_load(0);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) load(0, k);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) store(0, k);
+        begin_load(1);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) load(1, k);
         __syncthreads();
-        fetch(0, 0, 0);
-        fetch_scales(0);
+#pragma unroll
+        for (int k = 0; k < READS; ++k) { fetch(0, 0, 0, k); fetch_scale(0, k); }
         take_scales();
+        constexpr int MM = TI * TJ, EARLY = MM / 2 > 0 ? MM / 2 : 1;
         // panels behind the last one read as zeros and nothing of memory (every offset is out of its descriptor's range), so the loop
         // needs no case for its end
         for (int pn = 0; pn < panels; ++pn) {
-            fetch(pn, 1, 1);
-            MX_STEP(0, 0)
-            fetch(pn, 2, 0);
-            store(pn + 1);
-            MX_STEP(1, 1)
-            fetch(pn, 3, 1);
-            load(pn + 2);
-            MX_STEP(2, 0)
+            MX_STEP(0, 0, READS, EARLY, fetch(pn, 1, 1, k);)
+            MX_STEP(1, 1, READS + ITEMS, MM, if (k < READS) fetch(pn, 2, 0, k); else store(pn + 1, k - READS);)
+            begin_load(pn + 2);
+            MX_STEP(2, 0, READS + ITEMS, MM, if (k < READS) fetch(pn, 3, 1, k); else load(pn + 2, k - READS);)
             __syncthreads();
-            fetch(pn + 1, 0, 0);
-            fetch_scales(pn + 1);
-            MX_STEP(3, 1)
+            MX_STEP(3, 1, 2 * READS, EARLY, if (k < READS) fetch_scale(pn + 1, k); else fetch(pn + 1, 0, 0, k - READS);)
             take_scales();
         }
     }
 #undef MX_STEP
 
-    // ---- epilogue: strips of 32 rows go through the wave's own part of LDS, so that bias, activation and residual are one loop over
-    //      rows and the result leaves in runs along its rows
-    constexpr int COLS = TJ * 32, PITCH = COLS + 4;
-    static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "strips fit in the panels' LDS");
-    __syncthreads();
-    float *strip = reinterpret_cast<float *>(smem) + wave * 32 * PITCH;
-    for (int t = 0; t < TI; ++t) {
+    if constexpr (CONV) {
+        // ---- epilogue in D's layout: neighbouring lanes hold neighbouring positions of a plane
+        const int area = p.OH * p.OW, image0 = (j0 + wj0) / area;
+        const int64_t planes = (int64_t)I * area * 4;
+        const __amdgpu_buffer_rsrc_t out = resource(p.out ? p.out : p.a_codes, p.out ? image0 * planes : 0, p.out ? (p.batch - image0) * planes : 0);
+        const __amdgpu_buffer_rsrc_t residual = resource(p.residual ? p.residual : p.a_codes, p.residual ? image0 * planes : 0, p.residual ? (p.batch - image0) * planes : 0);
 #pragma unroll
-        for (int ti = 0; ti < TI; ++ti)
-            if (t == ti) {
+        for (int tj = 0; tj < TJ; ++tj) {
+            const int j = j0 + wj0 + tj * 32 + l31, image = j / area;
+            const int at = (int)((unsigned)(image - image0) * (unsigned)planes + (unsigned)(j - image * area) * 4u);
 #pragma unroll
-                for (int tj = 0; tj < TJ; ++tj)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) strip[(8 * (e / 4) + 4 * half + e % 4) * PITCH + tj * 32 + l31] = acc[ti][tj][e];
+            for (int ti = 0; ti < TI; ++ti) {
+                const int ib = i0 + wi0 + ti * 32;
+                if (ib < I) mx_finish_planes<RARE>(p, acc[ti][tj], ib, j, j < J, half, out, residual, at);
+                __builtin_amdgcn_sched_barrier(0);         // one tile's addresses and addends at a time
             }
-        const int ib = i0 + wi0 + t * 32;
-        if (ib < I) {
-            if constexpr (CONV) mx_finish_planes<COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
-            else mx_finish_rows<TYPE, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
+        }
+    } else {
+        // ---- epilogue: strips of 32 rows go through the wave's own part of LDS, so that the result leaves in whole vectors along its rows
+        constexpr int COLS = TJ * 32, PITCH = COLS + 4;
+        static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "strips fit in the panels' LDS");
+        __syncthreads();
+        float *strip = reinterpret_cast<float *>(smem) + wave * 32 * PITCH;
+        constexpr int VEC = MX_VEC<TYPE>;
+        const bool wide = p.J % VEC == 0 && p.out_stride % VEC == 0 && (uintptr_t)p.out % 16 == 0 &&
+                          (!p.residual || (p.residual_stride % VEC == 0 && (uintptr_t)p.residual % 16 == 0));
+#pragma unroll 1
+        for (int t = 0; t < TI; ++t) {
+#pragma unroll
+            for (int ti = 0; ti < TI; ++ti)
+                if (t == ti) {
+#pragma unroll
+                    for (int tj = 0; tj < TJ; ++tj)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) strip[(8 * (e / 4) + 4 * half + e % 4) * PITCH + tj * 32 + l31] = acc[ti][tj][e];
+                }
+            const int ib = i0 + wi0 + t * 32;
+            if (ib < I && wide) mx_finish_rows<TYPE, RARE, !RARE, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
+            else if (ib < I) mx_finish_rows<TYPE, RARE, false, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
         }
     }
 }
 
-template <int TYPE, bool CONV, bool BYTES, int TI, int TJ>
+template <int TYPE, bool CONV, bool BYTES, bool RARE, int TI, int TJ>
 static int launch_tile(const MxProductArgs &a, hipStream_t s)
 {
-    MxTileDev d{a, (int)((a.I + 64 * TI - 1) / (64 * TI)), (int)((a.J + 64 * TJ - 1) / (64 * TJ))};
+    MxTileDev d{a, (int)((a.I + 64 * TI - 1) / (64 * TI)), (int)((a.J + 64 * TJ - 1) / (64 * TJ)), a.G > 1 ? (unsigned)((0x100000000ull + a.G - 1) / a.G) : 0u};
     const int64_t grid = (int64_t)d.tiles_i * d.tiles_j;
     if (grid > 0x7fffffffLL) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((mx_product_tile_kernel<TYPE, CONV, BYTES, TI, TJ>), dim3((unsigned)grid), dim3(MX_THREADS), 0, s, d);
+    hipLaunchKernelGGL((mx_product_tile_kernel<TYPE, CONV, BYTES, RARE, TI, TJ>), dim3((unsigned)grid), dim3(MX_THREADS), 0, s, d);
     return (int)hipGetLastError();
 }
 
-// The tile by the size of D: the largest whose grid still gives every CU a workgroup.
+// The tile, measured on MI355X (GPU time, both sides of each border):
+//   rows    256 x 256 from k = 2048 on where it gives every CU a workgroup: 8192^3 320 us against 396 with 128 x 128 tiles, 8192 x 8192 x
+//           1024 98 against 92 (one workgroup a CU hides neither end of a tile behind another)
+//           128 x 128 where it gives every CU two workgroups, 64 x 128 where it gives every CU one (512 x 4096 x 4096: 14.5 us against 19.8
+//           with 128 x 128 and 15.0 with 64 x 64), else 64 x 64 (1001 x 1237 x 1511: 9.9 against 11.3)
+//   planes  64 x 128 where it gives every CU two workgroups, else 64 x 64: bound by the map's and the result's bytes and by the latency of
+//           gathering, they want waves (76 x 76 256 -> 128 1x1 of 64 images: 0.091 ms against 0.103 with 128 x 128 and 0.445 with 256 x 256)
 template <int TYPE, bool CONV, bool BYTES>
 static int launch_by_size(const MxProductArgs &a, hipStream_t s, char *name, size_t name_len)
 {
-    auto grid = [&](int64_t t) { return (a.I + t - 1) / t * ((a.J + t - 1) / t); };
-    const int cus = device_cu_count();
-    const int t = grid(256) >= cus ? 256 : grid(128) >= cus ? 128 : 64;
-    if (name) snprintf(name, name_len, "mx_product<%dx%d>", t, t);
-    if (t == 256) return launch_tile<TYPE, CONV, BYTES, 4, 4>(a, s);
-    if (t == 128) return launch_tile<TYPE, CONV, BYTES, 2, 2>(a, s);
-    return launch_tile<TYPE, CONV, BYTES, 1, 1>(a, s);
+    auto grid = [&](int64_t ti, int64_t tj) { return (a.I + 64 * ti - 1) / (64 * ti) * ((a.J + 64 * tj - 1) / (64 * tj)); };
+    const int64_t cus = device_cu_count();
+    const bool rare = a.act != YL_LINEAR && a.act != YL_LEAKY && a.act != YL_RELU;
+    int t = 11;
+    if (!rare) {
+        if (CONV) t = grid(1, 2) >= 2 * cus ? 12 : 11;
+        else t = grid(4, 4) >= cus && a.kb >= 64 ? 44 : grid(2, 2) >= 2 * cus ? 22 : grid(1, 2) >= cus ? 12 : 11;
+    }
+    if (name) snprintf(name, name_len, "mx_product<%dx%d>", t / 10 * 64, t % 10 * 64);
+    if (rare) return launch_tile<TYPE, CONV, BYTES, true, 1, 1>(a, s);
+    if constexpr (!CONV) {
+        if (t == 44) return launch_tile<TYPE, CONV, BYTES, false, 4, 4>(a, s);
+        if (t == 22) return launch_tile<TYPE, CONV, BYTES, false, 2, 2>(a, s);
+    }
+    if (t == 12) return launch_tile<TYPE, CONV, BYTES, false, 1, 2>(a, s);
+    return launch_tile<TYPE, CONV, BYTES, false, 1, 1>(a, s);
 }
 
 template <int TYPE, bool CONV>
