@@ -88,6 +88,17 @@ __device__ __forceinline__ unsigned mx_codes8(const float *v, unsigned byte)
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], s, 3);
     return q;
 }
+// eight codes -> the values they stand for; NaN under scale byte 255
+__device__ __forceinline__ void mx_values8(unsigned codes, unsigned byte, float *v)
+{
+    const float s = __builtin_bit_cast(float, byte << 23);
+    const mx_f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 1);
+    const mx_f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, s, 3);
+    v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1]; v[4] = c[0]; v[5] = c[1]; v[6] = d[0]; v[7] = d[1];
+    if (byte == 255)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = __builtin_nanf("");
+}
 __device__ __forceinline__ unsigned mx_abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
 __device__ __forceinline__ mx_v8i mx_operand(mx_v4i c) { return mx_v8i{c[0], c[1], c[2], c[3], 0, 0, 0, 0}; }

@@ -1,95 +1,215 @@
 // mx_quant.hip -- K14: ordinary tensors <-> MXFP4 (yl_mx_quantize, yl_mx_dequantize; formats in include/yolo2_hip.h).
 //
 // A block of 32 values along k: m = max |x|, S = 2^(floor(log2 m) - 2), codes = RNE_E2M1(x / S) saturated at 6.  Pure data movement:
-// bound by the bytes of the ordinary tensor (4 or 2 a value) and of the codes (17/32).
+// bound by the bytes of the ordinary tensor (4 or 2 a value) and of the codes (17/32).  Two forms of each direction:
+//   rows     k is contiguous: four neighbouring lanes hold a block, eight values each, read as 16-byte vectors; the block's maximum is
+//            taken across the four, each makes the 32 bits of its own codes, so a wave reads and writes contiguous memory
+//   columns  any other strides, in practice NCHW maps, where rows (pixels) are contiguous: a lane holds a whole block of one row, so a
+//            wave reads 64 neighbouring pixels of a channel at a time; codes go through LDS, so that a row's blocks leave together
 #include "mx_device.h"
 #include "mx.h"
 
 namespace yl {
 
-// one thread a block
+// vectors where memory has no more than the type's alignment: the hardware takes them
+typedef mx_u32x4 mx_u32x4_any __attribute__((aligned(2)));
+
+// eight values from x[i], the first `n` of them; 16 bytes at a time where all eight are there
 template <int TYPE>
-__global__ __launch_bounds__(256) void mx_quantize_kernel(MxDense s, uint4 *__restrict__ codes, unsigned char *__restrict__ scales, int64_t ld, int64_t kb)
+__device__ __forceinline__ void mx_read8(const void *x, int64_t i, int n, float *v)
 {
-    const int64_t n = s.batch * s.rows * kb;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-        const int64_t row = t / kb, j = t - row * kb;
-        const int64_t b = row / s.rows, r = row - b * s.rows;
-        const int64_t at = b * s.batch_stride + r * s.row_stride + j * MX_BLOCK * s.k_stride;
-        float v[MX_BLOCK];
+    if (n >= 8) {
+        const char *p = reinterpret_cast<const char *>(x) + i * (16 / MX_VEC<TYPE>);
+        if constexpr (TYPE == YL_F32) {
+            mx_unpack<TYPE>(*reinterpret_cast<const mx_u32x4_any *>(p), v);
+            mx_unpack<TYPE>(*reinterpret_cast<const mx_u32x4_any *>(p + 16), v + 4);
+        } else mx_unpack<TYPE>(*reinterpret_cast<const mx_u32x4_any *>(p), v);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < n ? mx_load<TYPE>(x, i + q) : 0.f;
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void mx_write8(void *x, int64_t i, int n, const float *v)
+{
+    if (n >= 8) {
+        char *p = reinterpret_cast<char *>(x) + i * (16 / MX_VEC<TYPE>);
+        *reinterpret_cast<mx_u32x4_any *>(p) = mx_pack<TYPE>(v);
+        if constexpr (TYPE == YL_F32) *reinterpret_cast<mx_u32x4_any *>(p + 16) = mx_pack<TYPE>(v + 4);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < n) mx_store<TYPE>(x, i + q, v[q]);
+    }
+}
+
+// INDEX: 32 bits while all blocks can be counted in them (a division of 64 bits costs more than the block)
+template <int TYPE, typename INDEX>
+__global__ __launch_bounds__(256) void mx_quantize_rows_kernel(MxDense s, unsigned *__restrict__ codes, unsigned char *__restrict__ scales, int64_t ld, INDEX kb, INDEX n)
+{
+    const int part = threadIdx.x & 3;
+    for (INDEX t = (INDEX)blockIdx.x * 64 + threadIdx.x / 4; t < n; t += (INDEX)gridDim.x * 64) {
+        const INDEX row = t / kb, j = t - row * kb;
+        int64_t at = (int64_t)row * s.row_stride;
+        if (s.batch > 1) {
+            const INDEX b = row / (INDEX)s.rows;
+            at = (int64_t)b * s.batch_stride + (int64_t)(row - b * (INDEX)s.rows) * s.row_stride;
+        }
+        const int64_t first = (int64_t)j * MX_BLOCK + part * 8, left = s.k - first;
+        float v[8];
+        mx_read8<TYPE>(s.data, at + first, left > 8 ? 8 : (int)left, v);
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < MX_BLOCK; ++i) {
-            v[i] = j * MX_BLOCK + i < s.k ? mx_load<TYPE>(s.data, at + i * s.k_stride) : 0.f;
-            top = max(top, mx_abs_bits(v[i]));
-        }
+        for (int q = 0; q < 8; ++q) top = max(top, mx_abs_bits(v[q]));
+        top = max(top, (unsigned)__shfl_xor((int)top, 1));
+        top = max(top, (unsigned)__shfl_xor((int)top, 2));
         const unsigned byte = mx_scale_byte(top);
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (byte != 255) q = make_uint4(mx_codes8(v, byte), mx_codes8(v + 8, byte), mx_codes8(v + 16, byte), mx_codes8(v + 24, byte));
-        codes[row * ld + j] = q;
-        scales[row * ld + j] = (unsigned char)byte;
+        codes[((int64_t)row * ld + j) * 4 + part] = byte == 255 ? 0u : mx_codes8(v, byte);
+        if (part == 0) scales[(int64_t)row * ld + j] = (unsigned char)byte;
+    }
+}
+
+template <int TYPE, typename INDEX>
+__global__ __launch_bounds__(256) void mx_dequantize_rows_kernel(const unsigned *__restrict__ codes, const unsigned char *__restrict__ scales, int64_t ld, MxDense d, INDEX kb, INDEX n)
+{
+    const int part = threadIdx.x & 3;
+    for (INDEX t = (INDEX)blockIdx.x * 64 + threadIdx.x / 4; t < n; t += (INDEX)gridDim.x * 64) {
+        const INDEX row = t / kb, j = t - row * kb;
+        int64_t at = (int64_t)row * d.row_stride;
+        if (d.batch > 1) {
+            const INDEX b = row / (INDEX)d.rows;
+            at = (int64_t)b * d.batch_stride + (int64_t)(row - b * (INDEX)d.rows) * d.row_stride;
+        }
+        const int64_t first = (int64_t)j * MX_BLOCK + part * 8, left = d.k - first;
+        if (left <= 0) continue;
+        const unsigned byte = scales[(int64_t)row * ld + j];
+        float v[8];
+        mx_values8(codes[((int64_t)row * ld + j) * 4 + part], byte, v);
+        mx_write8<TYPE>(const_cast<void *>(d.data), at + first, left > 8 ? 8 : (int)left, v);
+    }
+}
+
+// A workgroup takes 64 rows by 8 blocks, a wave two of the blocks.
+constexpr int MX_COLS_ROWS = 64, MX_COLS_BLOCKS = 8;
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void mx_quantize_columns_kernel(MxDense s, uint4 *__restrict__ codes, unsigned char *__restrict__ scales, int64_t ld, int64_t kb, int64_t groups)
+{
+    __shared__ uint4 lc[MX_COLS_ROWS * MX_COLS_BLOCKS];
+    __shared__ unsigned char ls[MX_COLS_ROWS * MX_COLS_BLOCKS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t tile = blockIdx.x / groups, j0 = (blockIdx.x - tile * groups) * MX_COLS_BLOCKS;
+    const int64_t row0 = tile * MX_COLS_ROWS, rows = s.batch * s.rows, row = row0 + lane;
+    const int blocks = (int)min((int64_t)MX_COLS_BLOCKS, kb - j0), count = (int)min((int64_t)MX_COLS_ROWS, rows - row0);
+    if (lane < count) {
+        const int64_t b = s.batch > 1 ? row / s.rows : 0;
+        const int64_t at = b * s.batch_stride + (row - b * s.rows) * s.row_stride;
+#pragma unroll
+        for (int h = 0; h < MX_COLS_BLOCKS / 4; ++h) {
+            const int j = wave + 4 * h;
+            if (j >= blocks) break;
+            const int64_t k0 = (j0 + j) * MX_BLOCK;
+            float v[MX_BLOCK];
+            if (k0 + MX_BLOCK <= s.k) {
+#pragma unroll
+                for (int i = 0; i < MX_BLOCK; ++i) v[i] = mx_load<TYPE>(s.data, at + (k0 + i) * s.k_stride);
+            } else {
+#pragma unroll
+                for (int i = 0; i < MX_BLOCK; ++i) v[i] = k0 + i < s.k ? mx_load<TYPE>(s.data, at + (k0 + i) * s.k_stride) : 0.f;
+            }
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < MX_BLOCK; ++i) top = max(top, mx_abs_bits(v[i]));
+            const unsigned byte = mx_scale_byte(top);
+            uint4 q = make_uint4(0, 0, 0, 0);
+            if (byte != 255) q = make_uint4(mx_codes8(v, byte), mx_codes8(v + 8, byte), mx_codes8(v + 16, byte), mx_codes8(v + 24, byte));
+            lc[lane * blocks + j] = q;
+            ls[lane * blocks + j] = (unsigned char)byte;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < count * blocks; i += 256) {
+        const int r = i / blocks;
+        const int64_t to = (row0 + r) * ld + j0 + (i - r * blocks);
+        codes[to] = lc[i];
+        scales[to] = ls[i];
     }
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint4 *__restrict__ codes, const unsigned char *__restrict__ scales, int64_t ld, MxDense d, int64_t kb)
+__global__ __launch_bounds__(256) void mx_dequantize_columns_kernel(const uint4 *__restrict__ codes, const unsigned char *__restrict__ scales, int64_t ld, MxDense d, int64_t kb, int64_t groups)
 {
-    const int64_t n = d.batch * d.rows * kb;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-        const int64_t row = t / kb, j = t - row * kb;
-        const int64_t b = row / d.rows, r = row - b * d.rows;
-        const int64_t at = b * d.batch_stride + r * d.row_stride + j * MX_BLOCK * d.k_stride;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t tile = blockIdx.x / groups, j0 = (blockIdx.x - tile * groups) * MX_COLS_BLOCKS;
+    const int64_t row = tile * MX_COLS_ROWS + lane;
+    if (row >= d.batch * d.rows) return;
+    const int64_t b = d.batch > 1 ? row / d.rows : 0;
+    const int64_t at = b * d.batch_stride + (row - b * d.rows) * d.row_stride;
+    for (int64_t j = j0 + wave; j < kb && j < j0 + MX_COLS_BLOCKS; j += 4) {
         const uint4 q = codes[row * ld + j];
         const unsigned byte = scales[row * ld + j];
-        const float s = __builtin_bit_cast(float, byte << 23);
         const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int i = 0; i < MX_BLOCK; i += 2) {
-            const mx_f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i / 8] >> (4 * (i % 8)), s, 0);
+        for (int g = 0; g < 4; ++g) {
+            float v[8];
+            mx_values8(w[g], byte, v);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (j * MX_BLOCK + i + e < d.k)
-                    mx_store<TYPE>(const_cast<void *>(d.data), at + (i + e) * d.k_stride, byte == 255 ? __builtin_nanf("") : v[e]);
+            for (int i = 0; i < 8; ++i) {
+                const int64_t k = j * MX_BLOCK + 8 * g + i;
+                if (k < d.k) mx_store<TYPE>(const_cast<void *>(d.data), at + k * d.k_stride, v[i]);
+            }
         }
     }
 }
 
-static unsigned mx_blocks_for(int64_t n)
+template <int TYPE>
+static int launch_quantize(const MxDense &src, void *codes, void *scales, int64_t ld, hipStream_t s)
 {
-    const int64_t g = (n + 255) / 256;
-    return (unsigned)(g < 1 ? 1 : (g > 256 * 64 ? 256 * 64 : g));
+    const int64_t kb = (src.k + MX_BLOCK - 1) / MX_BLOCK, rows = src.batch * src.rows, n = rows * kb;
+    if (src.k_stride == 1 || src.k == 1) {
+        const int64_t g = (n + 63) / 64;
+        const dim3 grid((unsigned)(g > 1 << 20 ? 1 << 20 : g));
+        if (n < 0x60000000) hipLaunchKernelGGL((mx_quantize_rows_kernel<TYPE, unsigned>), grid, dim3(256), 0, s, src, (unsigned *)codes, (unsigned char *)scales, ld, (unsigned)kb, (unsigned)n);
+        else hipLaunchKernelGGL((mx_quantize_rows_kernel<TYPE, int64_t>), grid, dim3(256), 0, s, src, (unsigned *)codes, (unsigned char *)scales, ld, kb, n);
+    } else {
+        const int64_t groups = (kb + MX_COLS_BLOCKS - 1) / MX_COLS_BLOCKS, g = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS * groups;
+        if (g > 0x7fffffff) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((mx_quantize_columns_kernel<TYPE>), dim3((unsigned)g), dim3(256), 0, s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
+    }
+    return (int)hipGetLastError();
+}
+
+template <int TYPE>
+static int launch_dequantize(const void *codes, const void *scales, int64_t ld, const MxDense &dst, hipStream_t s)
+{
+    const int64_t kb = (dst.k + MX_BLOCK - 1) / MX_BLOCK, rows = dst.batch * dst.rows, n = rows * kb;
+    if (dst.k_stride == 1 || dst.k == 1) {
+        const int64_t g = (n + 63) / 64;
+        const dim3 grid((unsigned)(g > 1 << 20 ? 1 << 20 : g));
+        if (n < 0x60000000) hipLaunchKernelGGL((mx_dequantize_rows_kernel<TYPE, unsigned>), grid, dim3(256), 0, s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, (unsigned)kb, (unsigned)n);
+        else hipLaunchKernelGGL((mx_dequantize_rows_kernel<TYPE, int64_t>), grid, dim3(256), 0, s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, kb, n);
+    } else {
+        const int64_t groups = (kb + MX_COLS_BLOCKS - 1) / MX_COLS_BLOCKS, g = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS * groups;
+        if (g > 0x7fffffff) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((mx_dequantize_columns_kernel<TYPE>), dim3((unsigned)g), dim3(256), 0, s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
+    }
+    return (int)hipGetLastError();
 }
 
 int launch_mx_quantize(const MxDense &src, void *codes, void *scales, int64_t ld, void *stream)
 {
-    const int64_t kb = (src.k + MX_BLOCK - 1) / MX_BLOCK, n = src.batch * src.rows * kb;
-    if (n == 0) return 0;
-    const dim3 grid(mx_blocks_for(n)), block(256);
+    if (src.batch == 0 || src.rows == 0 || src.k == 0) return 0;
     hipStream_t s = (hipStream_t)stream;
-    uint4 *c = (uint4 *)codes;
-    unsigned char *e = (unsigned char *)scales;
-    switch (src.type) {
-    case YL_F32: hipLaunchKernelGGL(mx_quantize_kernel<YL_F32>, grid, block, 0, s, src, c, e, ld, kb); break;
-    case YL_F16: hipLaunchKernelGGL(mx_quantize_kernel<YL_F16>, grid, block, 0, s, src, c, e, ld, kb); break;
-    default: hipLaunchKernelGGL(mx_quantize_kernel<YL_BF16>, grid, block, 0, s, src, c, e, ld, kb); break;
-    }
-    return (int)hipGetLastError();
+    return src.type == YL_F32 ? launch_quantize<YL_F32>(src, codes, scales, ld, s)
+         : src.type == YL_F16 ? launch_quantize<YL_F16>(src, codes, scales, ld, s) : launch_quantize<YL_BF16>(src, codes, scales, ld, s);
 }
 
 int launch_mx_dequantize(const void *codes, const void *scales, int64_t ld, const MxDense &dst, void *stream)
 {
-    const int64_t kb = (dst.k + MX_BLOCK - 1) / MX_BLOCK, n = dst.batch * dst.rows * kb;
-    if (n == 0) return 0;
-    const dim3 grid(mx_blocks_for(n)), block(256);
+    if (dst.batch == 0 || dst.rows == 0 || dst.k == 0) return 0;
     hipStream_t s = (hipStream_t)stream;
-    const uint4 *c = (const uint4 *)codes;
-    const unsigned char *e = (const unsigned char *)scales;
-    switch (dst.type) {
-    case YL_F32: hipLaunchKernelGGL(mx_dequantize_kernel<YL_F32>, grid, block, 0, s, c, e, ld, dst, kb); break;
-    case YL_F16: hipLaunchKernelGGL(mx_dequantize_kernel<YL_F16>, grid, block, 0, s, c, e, ld, dst, kb); break;
-    default: hipLaunchKernelGGL(mx_dequantize_kernel<YL_BF16>, grid, block, 0, s, c, e, ld, dst, kb); break;
-    }
-    return (int)hipGetLastError();
+    return dst.type == YL_F32 ? launch_dequantize<YL_F32>(codes, scales, ld, dst, s)
+         : dst.type == YL_F16 ? launch_dequantize<YL_F16>(codes, scales, ld, dst, s) : launch_dequantize<YL_BF16>(codes, scales, ld, dst, s);
 }
 
 }  // namespace yl
