@@ -28,14 +28,16 @@ def _fail(what: str):
     raise YoloHipError("mx: " + what)
 
 
-def _tensor(t, name: str, device=None):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+def _tensor(t, name: str, device: Optional[int] = None) -> int:
+    """The index of the GPU that t is on; -> raises unless t is a tensor on a GPU (on `device`, if given) that needs no gradient."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _fail("%s is not a tensor on a GPU" % name)
-    if device is not None and t.device != device:
-        _fail("%s is on %s, not on %s" % (name, t.device, device))
+    at = t.get_device()
+    if device is not None and at != device:
+        _fail("%s is on cuda:%d, not on cuda:%d" % (name, at, device))
     if t.requires_grad and torch.is_grad_enabled():
         _fail("%s requires a gradient, and there is no backward pass: detach it, or call under torch.no_grad()" % name)
-    return t
+    return at
 
 
 def _type(t, name: str) -> int:
@@ -45,45 +47,70 @@ def _type(t, name: str) -> int:
     return code
 
 
+def _blocks(k: int) -> int:
+    return (k + 4 * BLOCK - 1) // (4 * BLOCK) * 4          # yl_mx_blocks
+
+
+# the current stream of a device as a number; the public way makes an object of it first, which takes longer than a launch
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 class Matrix:
     """rows x k values in MXFP4: codes uint8 [rows, 16 * ld], scales uint8 [rows, ld], ld >= ceil(k / 32) blocks a row."""
-    __slots__ = ("codes", "scales", "k", "_c")
+    __slots__ = ("k", "rows", "index", "_codes", "_scales", "_c")
 
     def __init__(self, codes, scales, k: int):
-        self.codes, self.scales, self.k = _tensor(codes, "codes"), _tensor(scales, "scales", codes.device), int(k)
+        self.index = _tensor(codes, "codes")
+        _tensor(scales, "scales", self.index)
+        self.k = k = int(k)
         if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
             _fail("codes and scales are two-dimensional uint8 tensors")
         rows, ld = scales.shape
         if codes.shape[0] != rows or codes.shape[1] != 16 * ld or not codes.is_contiguous() or not scales.is_contiguous():
             _fail("codes [rows, 16 * ld] and scales [rows, ld] are contiguous and of the same rows and blocks")
-        if self.k < 0 or ld < (self.k + BLOCK - 1) // BLOCK:
-            _fail("k = %d needs %d blocks, the matrix has %d" % (self.k, (self.k + BLOCK - 1) // BLOCK, ld))
-        self._c = MxMatrix(codes.data_ptr(), scales.data_ptr(), rows, self.k, ld)
+        if k < 0 or ld < (k + BLOCK - 1) // BLOCK:
+            _fail("k = %d needs %d blocks, the matrix has %d" % (k, (k + BLOCK - 1) // BLOCK, ld))
+        self.rows, self._codes, self._scales = rows, codes, scales
+        self._c = MxMatrix(codes.data_ptr(), scales.data_ptr(), rows, k, ld)
 
     @classmethod
     def empty(cls, rows: int, k: int, device) -> "Matrix":
-        ld = lib.yl_mx_blocks(k)
-        return cls(torch.empty(rows, 16 * ld, dtype=torch.uint8, device=device), torch.empty(rows, ld, dtype=torch.uint8, device=device), k)
+        """A matrix of yl_mx_blocks(k) blocks a row, nothing in it yet; codes and scales share an allocation."""
+        ld = _blocks(k)
+        self = cls.__new__(cls)
+        both = torch.empty(rows * ld * 17, dtype=torch.uint8, device=device)
+        at = both.data_ptr()
+        self.k, self.rows, self.index, self._codes, self._scales = k, rows, both.get_device(), both, None
+        self._c = MxMatrix(at, at + rows * ld * 16, rows, k, ld)
+        return self
+
+    def _views(self):
+        both, n, ld = self._codes, self.rows * self._c.ld, self._c.ld
+        self._codes, self._scales = both[:16 * n].view(self.rows, 16 * ld), both[16 * n:].view(self.rows, ld)
 
     @property
-    def rows(self) -> int:
-        return self.scales.shape[0]
+    def codes(self):
+        if self._scales is None:
+            self._views()
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._views()
+        return self._scales
 
     @property
     def device(self):
-        return self.codes.device
+        return self._codes.device
 
 
-def _matrix(m, name: str, device=None) -> Matrix:
+def _matrix(m, name: str, device: Optional[int] = None) -> int:
     if not isinstance(m, Matrix):
         _fail("%s is not an mx.Matrix" % name)
-    if device is not None and m.codes.device != device:
-        _fail("%s is on %s, not on %s" % (name, m.codes.device, device))
-    return m
-
-
-def _at(device):
-    return device.index, torch.cuda.current_stream(device).cuda_stream
+    if device is not None and m.index != device:
+        _fail("%s is on cuda:%d, not on cuda:%d" % (name, m.index, device))
+    return m.index
 
 
 def _rows_of(x, name: str) -> Dense:
@@ -115,24 +142,25 @@ def _map_of(x, name: str) -> Dense:
     return Dense(x.data_ptr(), kind, b, h * w, c, x.stride(0), x.stride(3) if w > 1 else x.stride(2), x.stride(1))
 
 
-def _quantize(src: Dense, device, out: Optional[Matrix]) -> Matrix:
-    rows = src.batch * src.rows
+def _quantize(src: Dense, device: int, out: Optional[Matrix]) -> Matrix:
     if out is None:
-        out = Matrix.empty(rows, src.k, device)
-    check(lib.yl_mx_quantize(*_at(device), _ref(src), _ref(_matrix(out, "out", device)._c)), "yl_mx_quantize")
+        out = Matrix.empty(src.batch * src.rows, src.k, device)
+    else:
+        _matrix(out, "out", device)
+    check(lib.yl_mx_quantize(device, _stream(device), _ref(src), _ref(out._c)), "yl_mx_quantize")
     return out
 
 
 def quantize(x, out: Optional[Matrix] = None) -> Matrix:
     """x [..., k], any strides -> Matrix of x.numel() / k rows."""
-    _tensor(x, "x")
-    return _quantize(_rows_of(x, "x"), x.device, out)
+    device = _tensor(x, "x")
+    return _quantize(_rows_of(x, "x"), device, out)
 
 
 def quantize_nchw(x, out: Optional[Matrix] = None) -> Matrix:
     """A map [batch, c, h, w] -> Matrix of batch * h * w rows of c values (conv2d's x)."""
-    _tensor(x, "x")
-    return _quantize(_map_of(x, "x"), x.device, out)
+    device = _tensor(x, "x")
+    return _quantize(_map_of(x, "x"), device, out)
 
 
 def quantize_filters(w) -> Matrix:
@@ -147,50 +175,59 @@ def quantize_filters(w) -> Matrix:
 
 
 def _dequantize(q: Matrix, out, dst: Dense):
-    check(lib.yl_mx_dequantize(*_at(q.device), _ref(q._c), _ref(dst)), "yl_mx_dequantize")
+    check(lib.yl_mx_dequantize(q.index, _stream(q.index), _ref(q._c), _ref(dst)), "yl_mx_dequantize")
     return out
 
 
 def dequantize(q: Matrix, dtype=torch.float32, out=None):
     """The values of q, [rows, k]."""
-    _matrix(q, "q")
+    device = _matrix(q, "q")
     if out is None:
-        out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
-    return _dequantize(q, out, _rows_of(_tensor(out, "out", q.device), "out"))
+        out = torch.empty(q.rows, q.k, dtype=dtype, device=device)
+    else:
+        _tensor(out, "out", device)
+    return _dequantize(q, out, _rows_of(out, "out"))
 
 
 def dequantize_nchw(q: Matrix, batch: int, h: int, w: int, dtype=torch.float32, out=None):
     """The values of a quantised map, [batch, q.k, h, w]."""
-    _matrix(q, "q")
+    device = _matrix(q, "q")
     if out is None:
-        out = torch.empty(batch, q.k, h, w, dtype=dtype, device=q.device)
-    return _dequantize(q, out, _map_of(_tensor(out, "out", q.device), "out"))
+        out = torch.empty(batch, q.k, h, w, dtype=dtype, device=device)
+    else:
+        _tensor(out, "out", device)
+    return _dequantize(q, out, _map_of(out, "out"))
 
 
-def _epilogue(n: int, device, bias, activation, residual) -> Optional[MxEpilogue]:
+def _epilogue(n: int, device: int, bias, activation, residual) -> Optional[MxEpilogue]:
     act = ACTIVATIONS.get(activation) if isinstance(activation, str) else activation
     if act is None or not isinstance(act, int):
         _fail("unknown activation %r" % (activation,))
+    b = r = None
     if bias is not None:
         _tensor(bias, "bias", device)
         if bias.dtype is not torch.float32 or bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous():
             _fail("bias is a contiguous float32 tensor of %d values" % n)
-    if bias is None and residual is None and act == 3:
+        b = bias.data_ptr()
+    if residual is not None:
+        r = residual.data_ptr()
+    elif b is None and act == 3:
         return None
-    return MxEpilogue(bias.data_ptr() if bias is not None else None, act, residual.data_ptr() if residual is not None else None,
-                      residual.stride(0) if residual is not None else 0)
+    return MxEpilogue(b, act, r, residual.stride(0) if r is not None else 0)
 
 
-def _linear_args(lead, m: int, w: Matrix, device, bias, activation, residual, dtype, out):
+def _linear_args(lead, m: int, w: Matrix, device: int, bias, activation, residual, dtype, out):
     n = w.rows
     if out is None:
-        out = torch.empty(*lead, n, dtype=dtype, device=device)
-    elif tuple(out.shape) != (*lead, n):
-        _fail("out is not %s" % ((*lead, n),))
-    y = _rows_of(_tensor(out, "out", device), "out")
+        out = torch.empty((*lead, n), dtype=dtype, device=device)
+    else:
+        _tensor(out, "out", device)
+        if tuple(out.shape) != (*lead, n):
+            _fail("out is not %s" % ((*lead, n),))
+    y = _rows_of(out, "out")
     if residual is not None:
         _tensor(residual, "residual", device)
-        if residual.dtype is not out.dtype or tuple(residual.shape) != (*lead, n):
+        if residual.dtype is not out.dtype or residual.shape != out.shape:
             _fail("residual has not the result's type and shape")
         if residual.dim() != 2:
             try:
@@ -204,24 +241,24 @@ def _linear_args(lead, m: int, w: Matrix, device, bias, activation, residual, dt
 
 def matmul(x: Matrix, w: Matrix, bias=None, activation="linear", residual=None, dtype=torch.float32, out=None):
     """activation(x w^T + bias) + residual, [x.rows, w.rows]."""
-    device = _matrix(x, "x").codes.device
+    device = _matrix(x, "x")
     _matrix(w, "w", device)
     out, y, e = _linear_args((x.rows,), x.rows, w, device, bias, activation, residual, dtype, out)
-    check(lib.yl_mx_matmul(*_at(device), _ref(x._c), _ref(w._c), _ref(e) if e is not None else None, _ref(y)), "yl_mx_matmul")
+    check(lib.yl_mx_matmul(device, _stream(device), _ref(x._c), _ref(w._c), None if e is None else _ref(e), _ref(y)), "yl_mx_matmul")
     return out
 
 
 def linear(x, w: Matrix, bias=None, activation="linear", residual=None, dtype=None, out=None):
     """matmul(quantize(x), w, ...) on x [..., k], the same bits; the result has x's leading axes and, unless `dtype` says otherwise,
     its type."""
-    device = _tensor(x, "x").device
+    device = _tensor(x, "x")
     _matrix(w, "w", device)
     xd = _rows_of(x, "x")
     m = xd.rows
-    out, y, e = _linear_args(tuple(x.shape[:-1]), m, w, device, bias, activation, residual, dtype or x.dtype, out)
+    out, y, e = _linear_args(x.shape[:-1], m, w, device, bias, activation, residual, dtype or x.dtype, out)
     need = lib.yl_mx_linear_workspace(m, xd.k)
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    check(lib.yl_mx_linear(*_at(device), _ref(xd), _ref(w._c), _ref(e) if e is not None else None, _ref(y),
+    check(lib.yl_mx_linear(device, _stream(device), _ref(xd), _ref(w._c), None if e is None else _ref(e), _ref(y),
                            ws.data_ptr() if need else None, need), "yl_mx_linear")
     return out
 
@@ -230,7 +267,7 @@ def conv2d(x: Matrix, filters: Matrix, batch: int, h: int, w: int, size: int, st
            activation="linear", residual=None, out=None, want: str = "float"):
     """The convolution of a quantised map with quantised filters.  `want`: "float" -> FP32 [batch, filters, oh, ow]; "mx" -> the next
     layer's Matrix of batch * oh * ow rows; "both" -> the pair."""
-    device = _matrix(x, "x").codes.device
+    device = _matrix(x, "x")
     _matrix(filters, "filters", device)
     if want not in ("float", "mx", "both"):
         _fail("want is \"float\", \"mx\" or \"both\"")
@@ -239,18 +276,20 @@ def conv2d(x: Matrix, filters: Matrix, batch: int, h: int, w: int, size: int, st
     n, oh, ow = filters.rows, (h + 2 * pad - size) // stride + 1, (w + 2 * pad - size) // stride + 1
     if residual is not None:
         _tensor(residual, "residual", device)
-        if residual.dtype is not torch.float32 or tuple(residual.shape) != (batch, n, oh, ow) or not residual.is_contiguous():
+        if residual.dtype is not torch.float32 or residual.shape != (batch, n, oh, ow) or not residual.is_contiguous():
             _fail("residual is a contiguous float32 tensor of the result's shape")
     if want == "mx":
         if out is not None:
             _fail("out is given, but want is \"mx\"")
     elif out is None:
         out = torch.empty(batch, n, oh, ow, dtype=torch.float32, device=device)
-    elif _tensor(out, "out", device).dtype is not torch.float32 or tuple(out.shape) != (batch, n, oh, ow) or not out.is_contiguous():
-        _fail("out is a contiguous float32 tensor of the result's shape")
+    else:
+        _tensor(out, "out", device)
+        if out.dtype is not torch.float32 or out.shape != (batch, n, oh, ow) or not out.is_contiguous():
+            _fail("out is a contiguous float32 tensor of the result's shape")
     q = Matrix.empty(batch * oh * ow, n, device) if want != "float" else None
     e = _epilogue(n, device, bias, activation, residual)
     shape = MxConv(batch, h, w, size, stride, pad)
-    check(lib.yl_mx_conv2d(*_at(device), _ref(x._c), _ref(filters._c), _ref(shape), _ref(e) if e is not None else None,
-                           out.data_ptr() if out is not None else None, _ref(q._c) if q is not None else None), "yl_mx_conv2d")
+    check(lib.yl_mx_conv2d(device, _stream(device), _ref(x._c), _ref(filters._c), _ref(shape), None if e is None else _ref(e),
+                           None if out is None else out.data_ptr(), None if q is None else _ref(q._c)), "yl_mx_conv2d")
     return q if want == "mx" else (out, q) if want == "both" else out
