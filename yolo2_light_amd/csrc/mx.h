@@ -24,7 +24,8 @@ struct MxProductArgs {
     const void *a_codes, *a_scales, *b_codes, *b_scales;
     int64_t a_ld, b_ld;
     int64_t I, J;
-    int64_t kb;                    // blocks of the summed axis
+    int64_t k = 0;                 // the summed axis (linear)
+    int64_t kb;                    // ... in blocks
     const float *bias;             // along j (linear) or along i (conv)
     int act;
     const void *residual;
@@ -40,8 +41,10 @@ struct MxProductArgs {
 };
 int launch_mx_product(const MxProductArgs &a, void *stream, char *name = nullptr, size_t name_len = 0);
 
-// the linear layer on an unrounded x (launch_mx_product's a_codes / a_scales / a_ld unused): launch_mx_linear_takes says whether
-// the product rounds x itself
+// few rows (mx_few.hip)
+bool mx_few_takes(int64_t rows);
+int launch_mx_few(const MxProductArgs &a, void *stream);
+// the linear layer on an ordinary x (launch_mx_product's a_codes / a_scales / a_ld unused), where mx_linear_fused(rows, k)
 bool mx_linear_fused(int64_t rows, int64_t k);
 int launch_mx_linear(const MxProductArgs &a, const MxDense &x, void *stream);
 

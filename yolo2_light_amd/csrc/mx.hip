@@ -145,7 +145,7 @@ const char *check_product(int64_t x_rows, int64_t x_k, const yl_mx_matrix *w, co
         if (!same && out.meets(r)) return "y overlaps the residual";
     }
     a->b_codes = w->codes; a->b_scales = w->scales; a->b_ld = w->ld;
-    a->I = x_rows; a->J = w->rows; a->kb = blocks_of(w->k);
+    a->I = x_rows; a->J = w->rows; a->k = w->k; a->kb = blocks_of(w->k);
     a->bias = e ? e->bias : nullptr; a->act = e ? e->activation : YL_LINEAR;
     a->residual = e ? e->residual : nullptr; a->residual_stride = e ? e->residual_stride : 0;
     a->out = y->data; a->out_stride = y->row_stride; a->type = y->type;

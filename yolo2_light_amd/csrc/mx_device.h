@@ -103,6 +103,22 @@ __device__ __forceinline__ unsigned mx_abs_bits(float v) { return __builtin_bit_
 
 __device__ __forceinline__ mx_v8i mx_operand(mx_v4i c) { return mx_v8i{c[0], c[1], c[2], c[3], 0, 0, 0, 0}; }
 
-// magnitude bits' maximum sorts NaN above Inf above every number, as unsigned integers do
+// vectors where memory has no more than the type's alignment: the hardware takes them
+typedef mx_u32x4 mx_u32x4_any __attribute__((aligned(2)));
 
+// eight values from x[i], the first `n` of them; 16 bytes at a time where all eight are there
+template <int TYPE>
+__device__ __forceinline__ void mx_read8(const void *x, int64_t i, int n, float *v)
+{
+    if (n >= 8) {
+        const char *p = reinterpret_cast<const char *>(x) + i * (16 / MX_VEC<TYPE>);
+        if constexpr (TYPE == YL_F32) {
+            mx_unpack<TYPE>(*reinterpret_cast<const mx_u32x4_any *>(p), v);
+            mx_unpack<TYPE>(*reinterpret_cast<const mx_u32x4_any *>(p + 16), v + 4);
+        } else mx_unpack<TYPE>(*reinterpret_cast<const mx_u32x4_any *>(p), v);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < n ? mx_load<TYPE>(x, i + q) : 0.f;
+    }
+}
 }  // namespace yl

@@ -16,8 +16,8 @@ namespace yl {
 
 // ------------------------------------------------------------------ tiles staged through LDS
 // A workgroup of four waves owns BI x BJ of D, a wave TI x TJ tiles of 32 x 32 of it.  The summed axis goes by panels of eight blocks (256
-// values): the panel's codes lie in LDS as [row][8 units of 16 bytes], unit u at place u ^ (row & 7), so the eight rows that a read
-// of one unit touches per cycle fall into different banks; its scales as [row][8 bytes].  Lanes 0-31 feed the matrix instruction units
+// values): the panel's codes lie in LDS as [row][8 units of 16 bytes], unit u at place u ^ (row / 2 & 7), so that one unit of sixteen
+// neighbouring rows lies in all 64 banks once (u ^ (row & 7) puts rows r and r + 8 together: 580 cycles of conflicts a panel of 256 x 256); its scales as [row][8 bytes].  Lanes 0-31 feed the matrix instruction units
 // 0-3, lanes 32-63 units 4-7: a row's four scales of a panel are then one word a lane, and the instruction picks the byte of the step.
 // Two panels in LDS and one in registers: while the instructions of panel p run, panel p + 1 is written to the other half of LDS and
 // panel p + 2 is requested from memory; operands of the next step are read one step ahead, across panels too, so the barrier of a panel
@@ -182,7 +182,7 @@ __device__ __forceinline__ void mx_tile_of(int bid, int nwg, int tiles_i, int ti
 }
 
 template <int TYPE, bool CONV, bool BYTES, bool RARE, int TI, int TJ>
-__global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 2) void mx_product_tile_kernel(MxTileDev d)
+__global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_product_tile_kernel(MxTileDev d)
 {
     constexpr int BI = 64 * TI, BJ = 64 * TJ;
     constexpr int APT = BI / 32, BPT = BJ / 32, SPT = (BI + BJ + 127) / 128;
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 2) void mx_product_ti
         if (row < BI) soff[e] = min(row, I - 1 - i0) * a_ld;
         else soff[e] = (int)((unsigned)b_row(min(row - BI, BJ - 1), sout[e]) * (unsigned)b_ld);
     }
-    const int code_at = (tid / 8) * 128 + ((unit ^ ((tid / 8) & 7)) * 16);
+    const int code_at = (tid / 8) * 128 + ((unit ^ ((tid / 16) & 7)) * 16);
 
     // ---- a convolution's blocks in the order (tap, channel block): of this thread's unit, stepped by a panel at a time
     auto tap_of = [&](int block) { return (int)__umulhi((unsigned)block, d.g_magic) + (p.G == 1 ? block : 0); };      // block / G
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 2) void mx_product_ti
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-    const int ar = (wi0 + l31) * 128, br = BI * 128 + (wj0 + l31) * 128, x7 = l31 & 7;
+    const int ar = (wi0 + l31) * 128, br = BI * 128 + (wj0 + l31) * 128, x7 = (l31 >> 1) & 7;
     mx_v4i af[2][TI], bf[2][TJ];
     int sa[TI], sb[TJ], sa_next[TI], sb_next[TJ];
     constexpr int READS = TI + TJ;
@@ -367,14 +367,14 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 2) void mx_product_ti
 #pragma unroll
         for (int k = 0; k < READS; ++k) { fetch(0, 0, 0, k); fetch_scale(0, k); }
         take_scales();
-        constexpr int MM = TI * TJ, EARLY = MM / 2 > 0 ? MM / 2 : 1;
+        constexpr int MM = TI * TJ, HALF = ITEMS / 2, EARLY = MM / 2 > 0 ? MM / 2 : 1;
         // panels behind the last one read as zeros and nothing of memory (every offset is out of its descriptor's range), so the loop
         // needs no case for its end
         for (int pn = 0; pn < panels; ++pn) {
             MX_STEP(0, 0, READS, EARLY, fetch(pn, 1, 1, k);)
-            MX_STEP(1, 1, READS + ITEMS, MM, if (k < READS) fetch(pn, 2, 0, k); else store(pn + 1, k - READS);)
             begin_load(pn + 2);
-            MX_STEP(2, 0, READS + ITEMS, MM, if (k < READS) fetch(pn, 3, 1, k); else load(pn + 2, k - READS);)
+            MX_STEP(1, 1, READS + HALF, MM, if (k < READS) fetch(pn, 2, 0, k); else { store(pn + 1, k - READS); load(pn + 2, k - READS); })
+            MX_STEP(2, 0, READS + ITEMS - HALF, MM, if (k < READS) fetch(pn, 3, 1, k); else { store(pn + 1, k - READS + HALF); load(pn + 2, k - READS + HALF); })
             __syncthreads();
             MX_STEP(3, 1, 2 * READS, EARLY, if (k < READS) fetch_scale(pn + 1, k); else fetch(pn + 1, 0, 0, k - READS);)
             take_scales();
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 2) void mx_product_ti
         }
     } else {
         // ---- epilogue: strips of 32 rows go through the wave's own part of LDS, so that the result leaves in whole vectors along its rows
-        constexpr int COLS = TJ * 32, PITCH = COLS + 4;
+        constexpr int COLS = TJ * 32, PITCH = COLS + 8;              // rows r and r + 4, written at once, are half the banks apart
         static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "strips fit in the panels' LDS");
         __syncthreads();
         float *strip = reinterpret_cast<float *>(smem) + wave * 32 * PITCH;
@@ -476,14 +476,12 @@ int launch_mx_product(const MxProductArgs &a, void *stream, char *name, size_t n
     if (a.I == 0 || a.J == 0) return 0;
     hipStream_t s = (hipStream_t)stream;
     if (a.conv) return launch_typed<YL_F32, true>(a, s, name, name_len);
+    if (mx_few_takes(a.I)) return launch_mx_few(a, stream);
     switch (a.type) {
     case YL_F32: return launch_typed<YL_F32, false>(a, s, name, name_len);
     case YL_F16: return launch_typed<YL_F16, false>(a, s, name, name_len);
     default: return launch_typed<YL_BF16, false>(a, s, name, name_len);
     }
 }
-
-bool mx_linear_fused(int64_t, int64_t) { return false; }
-int launch_mx_linear(const MxProductArgs &, const MxDense &, void *) { return (int)hipErrorInvalidValue; }
 
 }  // namespace yl
