@@ -1,4 +1,4 @@
-// mx_few.hip -- K15f: products of MXFP4 matrices with few rows on one side (yl_mx_matmul and yl_mx_linear up to 64 rows of x; the single
+// mx_few.hip -- K15f: products of MXFP4 matrices with few rows on one side (yl_mx_matmul and yl_mx_linear up to 32 rows of x; the single
 // token of a decoding step).
 //
 // With few rows the product is a reading of w: 17/32 bytes a weight, once.  What counts is that every CU has enough of w in flight, so
@@ -30,7 +30,7 @@ bool mx_linear_fused(int64_t rows, int64_t k)
 {
     return rows <= 16 && k <= (int64_t)1 << 20 && (rows <= 1 || rows * k <= 32768) && mx_few_lds(rows, k) <= MX_FEW_LDS;
 }
-bool mx_few_takes(int64_t rows) { return rows <= 64; }
+bool mx_few_takes(int64_t rows) { return rows <= 32; }
 
 typedef unsigned mx_u32_any __attribute__((aligned(1)));
 
@@ -93,7 +93,7 @@ __device__ __forceinline__ void mx_few_load(MxFewChunk<C> &f, const uint4 *codes
     }
 }
 
-// C rows by C columns, R times C rows; group: the lane's block of a step
+// C rows by C columns; group: the lane's block of a step
 template <int C, int S>
 __device__ __forceinline__ auto mx_few_mfma(const MxFewChunk<C> &a, const MxFewChunk<C> &b, int group, decltype(mx_f32x4{}) acc)
 {
@@ -110,10 +110,10 @@ __device__ __forceinline__ auto mx_few_mfma(const MxFewChunk<C> &a, const MxFewC
 template <int C> struct MxFewAcc { typedef mx_f32x16 type; };
 template <> struct MxFewAcc<16> { typedef mx_f32x4 type; };
 
-template <int TYPE, int C, int R, bool FUSED>
+template <int TYPE, int C, bool FUSED>
 __global__ __launch_bounds__(MX_FEW_THREADS) void mx_product_few_kernel(MxProductArgs p, MxDense x)
 {
-    constexpr int G = 64 / C, U = 4 * G, E = C * C / 64, SUMS = MX_FEW_WAVES * R * C * C * 4;
+    constexpr int G = 64 / C, U = 4 * G, E = C * C / 64, SUMS = MX_FEW_WAVES * C * C * 4;
     __shared__ __attribute__((aligned(16))) char lds[FUSED && MX_FEW_LDS > SUMS ? MX_FEW_LDS : SUMS];
     const int lane = threadIdx.x & 63, l = lane % C, group = lane / C;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -122,61 +122,50 @@ __global__ __launch_bounds__(MX_FEW_THREADS) void mx_product_few_kernel(MxProduc
     const int64_t j = min(j0 + l, J - 1);
     const uint4 *b_codes = (const uint4 *)p.b_codes + j * p.b_ld;
     const unsigned char *b_scales = (const unsigned char *)p.b_scales + j * p.b_ld;
-    MxFewChunk<C> b, b_next, a[R];
+    MxFewChunk<C> b, b_next, a;
     if (wave < chunks) mx_few_load<C>(b, b_codes, b_scales, wave, kb, group);
     const int kbp = (kb + 15) / 16 * 16;
-    const uint4 *a_codes[R];
-    const unsigned char *a_scales[R];
+    const uint4 *a_codes;
+    const unsigned char *a_scales;
     if constexpr (FUSED) {
         if (x.type == YL_F32) mx_few_round<YL_F32>(x, lds, kb, kbp);
         else if (x.type == YL_F16) mx_few_round<YL_F16>(x, lds, kb, kbp);
         else mx_few_round<YL_BF16>(x, lds, kb, kbp);
         __syncthreads();
         const int row = min(l, I - 1);
-        a_codes[0] = reinterpret_cast<const uint4 *>(lds) + row * (kbp + 1);
-        a_scales[0] = reinterpret_cast<const unsigned char *>(lds) + I * (kbp + 1) * 16 + row * kbp;
+        a_codes = reinterpret_cast<const uint4 *>(lds) + row * (kbp + 1);
+        a_scales = reinterpret_cast<const unsigned char *>(lds) + I * (kbp + 1) * 16 + row * kbp;
     } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = min(r * C + l, I - 1);
-            a_codes[r] = (const uint4 *)p.a_codes + row * p.a_ld;
-            a_scales[r] = (const unsigned char *)p.a_scales + row * p.a_ld;
-        }
+        const int64_t row = min(l, I - 1);
+        a_codes = (const uint4 *)p.a_codes + row * p.a_ld;
+        a_scales = (const unsigned char *)p.a_scales + row * p.a_ld;
     }
-    typename MxFewAcc<C>::type acc[R];
+    typename MxFewAcc<C>::type acc;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[r][e] = 0.f;
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
     for (int c = wave; c < chunks; c += MX_FEW_WAVES) {
         if (c + MX_FEW_WAVES < chunks) mx_few_load<C>(b_next, b_codes, b_scales, c + MX_FEW_WAVES, kb, group);
-#pragma unroll
-        for (int r = 0; r < R; ++r) mx_few_load<C>(a[r], a_codes[r], a_scales[r], c, FUSED ? kbp : kb, group);     // LDS holds zeros up to kbp
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            acc[r] = mx_few_mfma<C, 0>(a[r], b, group, acc[r]);
-            acc[r] = mx_few_mfma<C, 1>(a[r], b, group, acc[r]);
-            acc[r] = mx_few_mfma<C, 2>(a[r], b, group, acc[r]);
-            acc[r] = mx_few_mfma<C, 3>(a[r], b, group, acc[r]);
-        }
+        mx_few_load<C>(a, a_codes, a_scales, c, FUSED ? kbp : kb, group);      // LDS holds zeros up to kbp
+        acc = mx_few_mfma<C, 0>(a, b, group, acc);
+        acc = mx_few_mfma<C, 1>(a, b, group, acc);
+        acc = mx_few_mfma<C, 2>(a, b, group, acc);
+        acc = mx_few_mfma<C, 3>(a, b, group, acc);
         b = b_next;
     }
     float *sums = reinterpret_cast<float *>(lds);
     if constexpr (FUSED) __syncthreads();                  // every wave has read x
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int row = C == 16 ? 4 * group + e : 8 * (e / 4) + 4 * group + e % 4;
-            sums[((wave * R + r) * C + row) * C + l] = acc[r][e];
-        }
+    for (int e = 0; e < E; ++e) {
+        const int row = C == 16 ? 4 * group + e : 8 * (e / 4) + 4 * group + e % 4;
+        sums[(wave * C + row) * C + l] = acc[e];
+    }
     __syncthreads();
-    for (int t = threadIdx.x; t < R * C * C; t += MX_FEW_THREADS) {
+    for (int t = threadIdx.x; t < C * C; t += MX_FEW_THREADS) {
         const int i = t / C, jj = j0 + t % C;
         if (i >= I || jj >= J) continue;
         float v = sums[t];
 #pragma unroll
-        for (int w = 1; w < MX_FEW_WAVES; ++w) v += sums[w * R * C * C + t];
+        for (int w = 1; w < MX_FEW_WAVES; ++w) v += sums[w * C * C + t];
         if (p.bias) v += p.bias[jj];
         v = yl_act_epilogue(v, p.act);
         if (p.residual) v += mx_load<TYPE>(p.residual, (int64_t)i * p.residual_stride + jj);
@@ -184,14 +173,14 @@ __global__ __launch_bounds__(MX_FEW_THREADS) void mx_product_few_kernel(MxProduc
     }
 }
 
-template <int C, int R, bool FUSED>
+template <int C, bool FUSED>
 static int launch_few(const MxProductArgs &a, const MxDense &x, hipStream_t s)
 {
     const dim3 grid((unsigned)((a.J + C - 1) / C)), block(MX_FEW_THREADS);
     switch (a.type) {
-    case YL_F32: hipLaunchKernelGGL((mx_product_few_kernel<YL_F32, C, R, FUSED>), grid, block, 0, s, a, x); break;
-    case YL_F16: hipLaunchKernelGGL((mx_product_few_kernel<YL_F16, C, R, FUSED>), grid, block, 0, s, a, x); break;
-    default: hipLaunchKernelGGL((mx_product_few_kernel<YL_BF16, C, R, FUSED>), grid, block, 0, s, a, x); break;
+    case YL_F32: hipLaunchKernelGGL((mx_product_few_kernel<YL_F32, C, FUSED>), grid, block, 0, s, a, x); break;
+    case YL_F16: hipLaunchKernelGGL((mx_product_few_kernel<YL_F16, C, FUSED>), grid, block, 0, s, a, x); break;
+    default: hipLaunchKernelGGL((mx_product_few_kernel<YL_BF16, C, FUSED>), grid, block, 0, s, a, x); break;
     }
     return (int)hipGetLastError();
 }
@@ -201,15 +190,14 @@ int launch_mx_few(const MxProductArgs &a, void *stream)
     hipStream_t s = (hipStream_t)stream;
     // 16 columns a workgroup where 32 would leave CUs without one (16 x 4096 x 4096 4.9 us against 6.6; 16 x 16384 x 4096 12.6 against
     // 10.7), and where the fused form, which has no other, would run: its sums are these
-    if (a.I <= 16 && (a.J < 32 * (int64_t)device_cu_count() || mx_linear_fused(a.I, a.k))) return launch_few<16, 1, false>(a, MxDense{}, s);
-    if (a.I <= 32) return launch_few<32, 1, false>(a, MxDense{}, s);
-    return launch_few<32, 2, false>(a, MxDense{}, s);
+    if (a.I <= 16 && (a.J < 32 * (int64_t)device_cu_count() || mx_linear_fused(a.I, a.k))) return launch_few<16, false>(a, MxDense{}, s);
+    return launch_few<32, false>(a, MxDense{}, s);
 }
 
 int launch_mx_linear(const MxProductArgs &a, const MxDense &x, void *stream)
 {
     if (a.I == 0 || a.J == 0) return 0;
-    return launch_few<16, 1, true>(a, x, (hipStream_t)stream);
+    return launch_few<16, true>(a, x, (hipStream_t)stream);
 }
 
 }  // namespace yl

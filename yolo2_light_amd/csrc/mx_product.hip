@@ -163,10 +163,28 @@ __device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const m
     }
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication: with l = ceil(log2 d), m = ceil(2^(31 + l) / d) fits 32 bits and n m / 2^(31 + l) is at most
+// n / 2^(31 + l) < 1 / d above n / d
+struct MxDiv {
+    unsigned m = 0;
+    int shift = 0, d = 1;
+    MxDiv() = default;
+    explicit MxDiv(int64_t by) : d((int)by)
+    {
+        if (by <= 1) return;
+        int l = 0;
+        while (((int64_t)1 << l) < by) ++l;
+        m = (unsigned)((((uint64_t)1 << (31 + l)) + by - 1) / by);
+        shift = l - 1;
+    }
+    __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : (int)(__umulhi((unsigned)n, m) >> shift); }
+};
+
 struct MxTileDev {
     MxProductArgs p;
     int tiles_i, tiles_j;
-    unsigned g_magic;      // ceil(2^32 / G): block / G is the high half of the product while block * G < 2^32 (G = 1: 0)
+    MxDiv area, width, blocks;     // conv: positions of an image, positions of a line, blocks of a pixel
+    int size_magic;                // conv: tap / size = tap * size_magic >> 8 for taps below 32
 };
 
 // logical tile of a workgroup: every XCD (blockIdx % 8) gets one contiguous run of tiles, walked in bands of 8 tiles along i so that the
@@ -182,7 +200,7 @@ __device__ __forceinline__ void mx_tile_of(int bid, int nwg, int tiles_i, int ti
 }
 
 template <int TYPE, bool CONV, bool BYTES, bool RARE, int TI, int TJ>
-__global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_product_tile_kernel(MxTileDev d)
+__global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !BYTES ? 3 : 6 - TI - TJ) void mx_product_tile_kernel(MxTileDev d)
 {
     constexpr int BI = 64 * TI, BJ = 64 * TJ;
     constexpr int APT = BI / 32, BPT = BJ / 32, SPT = (BI + BJ + 127) / 128;
@@ -208,9 +226,8 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
     int64_t b_row0 = j0, b_rows = p.J - j0;            // the row that offset 0 of B's descriptors means, and rows from it to the end
     int cj_image = 0, cj_y = 0;                        // conv: image and first input line of the tile's first position
     if (CONV) {
-        const int area = p.OH * p.OW;
-        cj_image = j0 / area;
-        cj_y = (j0 - cj_image * area) / p.OW * p.stride;
+        cj_image = d.area(j0);
+        cj_y = d.width(j0 - cj_image * d.area.d) * p.stride;
         b_row0 = ((int64_t)cj_image * p.H + min(cj_y, p.H - 1)) * p.W - (int64_t)p.pad * p.W - p.pad;
         cj_y = min(cj_y, p.H - 1);
         b_rows = (int64_t)p.batch * p.H * p.W - b_row0;
@@ -226,12 +243,13 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
         const int j = min(j0 + jl, J - 1);
         outside = 0;
         if (!CONV) return j - j0;
-        const int area = p.OH * p.OW, image = j / area, pix = j - image * area, oy = pix / p.OW, ox = pix - oy * p.OW;
+        const int image = d.area(j), pix = j - image * d.area.d, oy = d.width(pix), ox = pix - oy * p.OW;
         const int y = oy * p.stride - p.pad, x = ox * p.stride - p.pad;
+        // columns of the filter from -x to W - x are inside, lines likewise
+        const unsigned columns = ((1u << min(max(p.W - x, 0), p.size)) - 1u) & (~0u << max(-x, 0));
         unsigned in = 0;
         for (int ky = 0; ky < p.size; ++ky)
-            for (int kx = 0; kx < p.size; ++kx)
-                if (y + ky >= 0 && y + ky < p.H && x + kx >= 0 && x + kx < p.W) in |= 1u << (ky * p.size + kx);
+            if ((unsigned)(y + ky) < (unsigned)p.H) in |= columns << (ky * p.size);
         outside = ~in;
         return ((image - cj_image) * p.H + y + p.pad - cj_y) * p.W + x + p.pad;
     };
@@ -245,28 +263,29 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
     for (int e = 0; e < SPT; ++e) {
         const int row = tid / 2 + 128 * e;
         sout[e] = 0;
-        if (row < BI) soff[e] = min(row, I - 1 - i0) * a_ld;
+        if (32 * wave + 128 * e < BI) soff[e] = min(row, I - 1 - i0) * a_ld;
         else soff[e] = (int)((unsigned)b_row(min(row - BI, BJ - 1), sout[e]) * (unsigned)b_ld);
     }
     const int code_at = (tid / 8) * 128 + ((unit ^ ((tid / 16) & 7)) * 16);
 
     // ---- a convolution's blocks in the order (tap, channel block): of this thread's unit, stepped by a panel at a time
-    auto tap_of = [&](int block) { return (int)__umulhi((unsigned)block, d.g_magic) + (p.G == 1 ? block : 0); };      // block / G
+    auto tap_of = [&](int block) { return d.blocks(block); };
     int tap = 0, g = 0, step_tap = 0, step_g = 0;
     if (CONV) {
         tap = tap_of(unit); g = unit - tap * p.G;
         step_tap = tap_of(MX_PANEL); step_g = MX_PANEL - step_tap * p.G;
     }
     auto tap_row = [&](int t) {                        // tap -> rows of the map from the first tap
-        const int ky = p.size == 3 ? (t * 11) >> 5 : (p.size == 1 ? 0 : t / p.size);
+        const int ky = t * d.size_magic >> 8;
         return ky * p.W + t - ky * p.size;
     };
     auto outside_bit = [](unsigned m, int t) { return __builtin_amdgcn_sbfe((int)m, t, 1); };
 
     // the panel's ITEMS requests and, in the same order, the stores of what they brought: one or two between two matrix instructions
     constexpr int ITEMS = APT + BPT + SPT;
-    mx_v4i areg[APT], breg[BPT];
-    int sreg[SPT][BYTES ? 4 : 1];
+    constexpr int SETS = TI + TJ > 4 || TI != TJ || BYTES ? 1 : 2;          // panels in registers: small tiles are over too soon for one to hide memory
+    mx_v4i areg[SETS][APT], breg[SETS][BPT];
+    int sreg[SETS][SPT][BYTES ? 4 : 1];
     int here = 0, here_out[BPT];                       // conv: this thread's unit of the panel being requested, rows outside the image as -1
     auto begin_load = [&](int pn) {                    // the panels in order, each once
         const int end = pn * MX_PANEL + unit >= kb ? -1 : 0;
@@ -279,16 +298,16 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
             if (g >= p.G) { g -= p.G; ++tap; }
         }
     };
-    auto load = [&](int pn, int k) {
+    auto load = [&](int pn, int set, int k) {
         const int at = pn * MX_PANEL * 16, end = pn * MX_PANEL + unit >= kb ? -1 : 0;
-        if (k < APT) areg[k] = __builtin_bit_cast(mx_v4i, __builtin_amdgcn_raw_buffer_load_b128(ra, aoff[k] | end, at, 0));
+        if (k < APT) areg[set][k] = __builtin_bit_cast(mx_v4i, __builtin_amdgcn_raw_buffer_load_b128(ra, aoff[k] | end, at, 0));
         else if (k < APT + BPT) {
             const int e = k - APT;
-            breg[e] = __builtin_bit_cast(mx_v4i, CONV ? __builtin_amdgcn_raw_buffer_load_b128(rb, (boff[e] + here) | here_out[e], 0, 0)
+            breg[set][e] = __builtin_bit_cast(mx_v4i, CONV ? __builtin_amdgcn_raw_buffer_load_b128(rb, (boff[e] + here) | here_out[e], 0, 0)
                                                       : __builtin_amdgcn_raw_buffer_load_b128(rb, boff[e] | end, at, 0));
         } else {
             const int e = k - APT - BPT, block0 = pn * MX_PANEL + 4 * word;            // the word's first block
-            const bool of_a = BI % 128 == 0 ? 128 * e < BI : tid / 2 + 128 * e < BI;
+            const bool of_a = 32 * wave + 128 * e < BI;                                // a wave brings 32 rows' words
             // the word, or its bytes one by one
 #pragma unroll
             for (int i = 0; i < (BYTES ? 4 : 1); ++i) {
@@ -298,20 +317,20 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
                     const int t = tap_of(block);
                     off = (soff[e] + tap_row(t) * b_ld + block - t * p.G) | outside_bit(sout[e], min(t, 31)) | off_end;
                 }
-                if constexpr (BYTES) sreg[e][i] = of_a ? __builtin_amdgcn_raw_buffer_load_b8(ras, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b8(rbs, off, 0, 0);
-                else sreg[e][i] = of_a ? __builtin_amdgcn_raw_buffer_load_b32(ras, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(rbs, off, 0, 0);
+                if constexpr (BYTES) sreg[set][e][i] = of_a ? __builtin_amdgcn_raw_buffer_load_b8(ras, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b8(rbs, off, 0, 0);
+                else sreg[set][e][i] = of_a ? __builtin_amdgcn_raw_buffer_load_b32(ras, off, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(rbs, off, 0, 0);
             }
         }
     };
-    auto store = [&](int pn, int k) {                  // registers -> the panel's half of LDS
+    auto store = [&](int pn, int set, int k) {                  // registers -> the panel's half of LDS
         char *st = smem + (pn & 1) * STAGE;
-        if (k < APT) *reinterpret_cast<mx_v4i *>(st + code_at + k * 4096) = areg[k];
-        else if (k < APT + BPT) *reinterpret_cast<mx_v4i *>(st + BI * 128 + code_at + (k - APT) * 4096) = breg[k - APT];
+        if (k < APT) *reinterpret_cast<mx_v4i *>(st + code_at + k * 4096) = areg[set][k];
+        else if (k < APT + BPT) *reinterpret_cast<mx_v4i *>(st + BI * 128 + code_at + (k - APT) * 4096) = breg[set][k - APT];
         else {
             const int e = k - APT - BPT, left = kb - (pn * MX_PANEL + 4 * word);
             const unsigned keep = left >= 4 ? 0xFFFFFFFFu : (left <= 0 ? 0u : (1u << (8 * left)) - 1u);     // scales behind the last block are not read
-            unsigned w = (unsigned)sreg[e][0];
-            if constexpr (BYTES) w = (w & 255u) | ((unsigned)sreg[e][1] & 255u) << 8 | ((unsigned)sreg[e][2] & 255u) << 16 | ((unsigned)sreg[e][3] & 255u) << 24;
+            unsigned w = (unsigned)sreg[set][e][0];
+            if constexpr (BYTES) w = (w & 255u) | ((unsigned)sreg[set][e][1] & 255u) << 8 | ((unsigned)sreg[set][e][2] & 255u) << 16 | ((unsigned)sreg[set][e][3] & 255u) << 24;
             if ((BI + BJ) % 128 == 0 || tid + 256 * e < 2 * (BI + BJ)) *reinterpret_cast<unsigned *>(st + (BI + BJ) * 128 + (tid + 256 * e) * 4) = w & keep;
         }
     };
@@ -357,40 +376,62 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
     if (panels > 0) {
         begin_load(0);
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k) load(0, k);
+        for (int k = 0; k < ITEMS; ++k) load(0, 0, k);
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k) store(0, k);
-        begin_load(1);
+        for (int set = 1; set < SETS; ++set) {
+            begin_load(set);
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k) load(1, k);
+            for (int k = 0; k < ITEMS; ++k) load(set, set, k);
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) store(0, 0, k);
+        begin_load(SETS);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) load(SETS, 0, k);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < READS; ++k) { fetch(0, 0, 0, k); fetch_scale(0, k); }
         take_scales();
         constexpr int MM = TI * TJ, HALF = ITEMS / 2, EARLY = MM / 2 > 0 ? MM / 2 : 1;
-        // panels behind the last one read as zeros and nothing of memory (every offset is out of its descriptor's range), so the loop
-        // needs no case for its end
-        for (int pn = 0; pn < panels; ++pn) {
-            MX_STEP(0, 0, READS, EARLY, fetch(pn, 1, 1, k);)
-            begin_load(pn + 2);
-            MX_STEP(1, 1, READS + HALF, MM, if (k < READS) fetch(pn, 2, 0, k); else { store(pn + 1, k - READS); load(pn + 2, k - READS); })
-            MX_STEP(2, 0, READS + ITEMS - HALF, MM, if (k < READS) fetch(pn, 3, 1, k); else { store(pn + 1, k - READS + HALF); load(pn + 2, k - READS + HALF); })
-            __syncthreads();
-            MX_STEP(3, 1, 2 * READS, EARLY, if (k < READS) fetch_scale(pn + 1, k); else fetch(pn + 1, 0, 0, k - READS);)
-            take_scales();
+        // Panel PN while panel PN + 1 lies in set SET of the registers: it is stored, and panel PN + 1 + SETS requested in its place.  Panels
+        // behind the last one read as zeros and nothing of memory (every offset is out of its descriptor's range), so the loop needs no
+        // case for its end.
+#define MX_PANEL_BODY(PN, SET)                                                                                                   \
+    {                                                                                                                            \
+        MX_STEP(0, 0, READS, EARLY, fetch(PN, 1, 1, k);)                                                                         \
+        begin_load((PN) + 1 + SETS);                                                                                             \
+        MX_STEP(1, 1, READS + HALF, MM,                                                                                          \
+                if (k < READS) fetch(PN, 2, 0, k); else { store((PN) + 1, SET, k - READS); load((PN) + 1 + SETS, SET, k - READS); }) \
+        MX_STEP(2, 0, READS + ITEMS - HALF, MM,                                                                                  \
+                if (k < READS) fetch(PN, 3, 1, k);                                                                               \
+                else { store((PN) + 1, SET, k - READS + HALF); load((PN) + 1 + SETS, SET, k - READS + HALF); })                  \
+        __syncthreads();                                                                                                         \
+        MX_STEP(3, 1, 2 * READS, EARLY, if (k < READS) fetch_scale((PN) + 1, k); else fetch((PN) + 1, 0, 0, k - READS);)         \
+        take_scales();                                                                                                           \
+    }
+        if constexpr (SETS == 1) {
+            for (int pn = 0; pn < panels; ++pn) MX_PANEL_BODY(pn, 0)
+        } else {
+            int pn = 0;
+            for (; pn + 1 < panels; pn += 2) {
+                MX_PANEL_BODY(pn, 1)
+                MX_PANEL_BODY(pn + 1, 0)
+            }
+            if (pn < panels) MX_PANEL_BODY(pn, 1)
         }
+#undef MX_PANEL_BODY
     }
 #undef MX_STEP
 
     if constexpr (CONV) {
         // ---- epilogue in D's layout: neighbouring lanes hold neighbouring positions of a plane
-        const int area = p.OH * p.OW, image0 = (j0 + wj0) / area;
+        const int area = d.area.d, image0 = d.area(j0 + wj0);
         const int64_t planes = (int64_t)I * area * 4;
         const __amdgpu_buffer_rsrc_t out = resource(p.out ? p.out : p.a_codes, p.out ? image0 * planes : 0, p.out ? (p.batch - image0) * planes : 0);
         const __amdgpu_buffer_rsrc_t residual = resource(p.residual ? p.residual : p.a_codes, p.residual ? image0 * planes : 0, p.residual ? (p.batch - image0) * planes : 0);
 #pragma unroll
         for (int tj = 0; tj < TJ; ++tj) {
-            const int j = j0 + wj0 + tj * 32 + l31, image = j / area;
+            const int j = j0 + wj0 + tj * 32 + l31, image = d.area(j);
             const int at = (int)((unsigned)(image - image0) * (unsigned)planes + (unsigned)(j - image * area) * 4u);
 #pragma unroll
             for (int ti = 0; ti < TI; ++ti) {
@@ -428,7 +469,13 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : 6 - TI - TJ) void mx_
 template <int TYPE, bool CONV, bool BYTES, bool RARE, int TI, int TJ>
 static int launch_tile(const MxProductArgs &a, hipStream_t s)
 {
-    MxTileDev d{a, (int)((a.I + 64 * TI - 1) / (64 * TI)), (int)((a.J + 64 * TJ - 1) / (64 * TJ)), a.G > 1 ? (unsigned)((0x100000000ull + a.G - 1) / a.G) : 0u};
+    MxTileDev d{a, (int)((a.I + 64 * TI - 1) / (64 * TI)), (int)((a.J + 64 * TJ - 1) / (64 * TJ)), MxDiv(), MxDiv(), MxDiv(), 0};
+    if (CONV) {
+        d.area = MxDiv((int64_t)a.OH * a.OW);
+        d.width = MxDiv(a.OW);
+        d.blocks = MxDiv(a.G);
+        d.size_magic = (256 + a.size - 1) / a.size;
+    }
     const int64_t grid = (int64_t)d.tiles_i * d.tiles_j;
     if (grid > 0x7fffffffLL) return (int)hipErrorInvalidValue;
     hipLaunchKernelGGL((mx_product_tile_kernel<TYPE, CONV, BYTES, RARE, TI, TJ>), dim3((unsigned)grid), dim3(MX_THREADS), 0, s, d);
