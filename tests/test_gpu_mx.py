@@ -529,6 +529,29 @@ def test_a_large_map(mx):
     close(got, want, tol)
 
 
+def at_the_end(t):
+    """t's values in the last bytes of an allocation of its own (32 MB: a segment of the allocator's, nothing behind it)."""
+    whole = torch.empty(32 << 20, dtype=torch.uint8, device="cuda")
+    end = whole[(32 << 20) - t.numel() * t.element_size():].view(t.dtype).view(t.shape)
+    end.copy_(t)
+    return end
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 48, 96), (5, 72, 160), (33, 64, 64), (40, 256, 160), (41, 261, 100), (129, 136, 96), (257, 1000, 64)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_behind_the_last_are_not_read(mx, m, n, k, dtype):
+    """A strip of 32 rows with fewer than a step's rows in it once read the residual of the rows behind them."""
+    x, w, b = at_the_end(rand(m, k, seed=1, dtype=dtype)), mx.quantize(rand(n, k, seed=2).cuda()), at_the_end(rand(n, seed=3))
+    w = mx.Matrix(at_the_end(w.codes), at_the_end(w.scales), k)
+    res = at_the_end(rand(m, n, seed=4, dtype=dtype))
+    y = mx.linear(x, w, bias=b, activation="leaky", residual=res, out=at_the_end(torch.zeros(m, n, dtype=TYPES[dtype])))
+    q = mx.quantize(x)
+    q = mx.Matrix(at_the_end(q.codes), at_the_end(q.scales), k)
+    assert torch.equal(y, mx.matmul(q, w, bias=b, activation="leaky", residual=res, dtype=TYPES[dtype]))
+    want, tol = o.product_tolerance(o.rounded(f64(x)), o.rounded(f64(rand(n, k, seed=2))), f64(b), "leaky", f64(res), dtype)
+    close(y, want, tol)
+
+
 def test_gradients_are_refused(mx):
     from yolo2_light_amd import YoloHipError
     w, _ = make(mx, 8, 32, 1)

@@ -58,6 +58,7 @@ __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const flo
 #pragma unroll
         for (int q = 0; q < VEC; ++q) bias[q] = p.bias ? p.bias[j + q] : 0.f;
         const int r0 = lane / LANES;
+        if (r0 >= rows) return;                            // and below: the first row of a step is always one of the matrix
         int64_t at = (int64_t)(ib + r0) * p.out_stride + j, res = (int64_t)(ib + r0) * p.residual_stride + j;
 #pragma unroll 1
         for (int step = 0; step < STEPS; step += AHEAD) {
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
     // ---- what this thread brings: units (row t / 8 + 32 e, unit t % 8) and scale words (row t / 2 + 128 e, word t % 2)
     const int unit = tid & 7, word = tid & 1;
     auto resource = [](const void *base, int64_t off, int64_t bytes) {
-        const int64_t n = bytes > 0xFFFFFFFELL ? 0xFFFFFFFELL : bytes;
+        const int64_t n = bytes > 0xFFFFFFFELL ? 0xFFFFFFFELL : bytes < 0 ? 0 : bytes;
         return __builtin_amdgcn_make_buffer_rsrc((void *)((const char *)base + off), 0, (int)(unsigned)n, 0x00020000);
     };
     const int64_t a_row0 = i0, a_rows = p.I - i0;
@@ -483,12 +484,15 @@ static int launch_tile(const MxProductArgs &a, hipStream_t s)
 }
 
 // The tile, measured on MI355X (GPU time, both sides of each border):
-//   rows    256 x 256 from k = 2048 on where it gives every CU a workgroup: 8192^3 320 us against 396 with 128 x 128 tiles, 8192 x 8192 x
-//           1024 98 against 92 (one workgroup a CU hides neither end of a tile behind another)
-//           128 x 128 where it gives every CU two workgroups, 64 x 128 where it gives every CU one (512 x 4096 x 4096: 14.5 us against 19.8
-//           with 128 x 128 and 15.0 with 64 x 64), else 64 x 64 (1001 x 1237 x 1511: 9.9 against 11.3)
+//   rows    256 x 256 from k = 2048 on where it gives every CU a workgroup: 4096 x 16384 x 4096 185 us against 209 with 128 x 128 tiles, but
+//           4096 x 4096 x 1024 27.3 against 25.3 (one workgroup a CU hides neither end of a tile behind another)
+//           128 x 128 where it gives every CU two workgroups, or one from k = 2048 on: 512 x 8192 x 8192 31.1 us against 43.5 with 64 x 128
+//           tiles, 1024 x 4096 x 512 9.3 against 8.5
+//           64 x 128 where it gives every CU one (512 x 4096 x 4096 13.9 us against 16.4 with 128 x 128 and 14.3 with 64 x 64)
+//           else 64 x 64 (1024^3 5.6 us against 7.2 with 64 x 128)
 //   planes  64 x 128 where it gives every CU two workgroups, else 64 x 64: bound by the map's and the result's bytes and by the latency of
-//           gathering, they want waves (76 x 76 256 -> 128 1x1 of 64 images: 0.091 ms against 0.103 with 128 x 128 and 0.445 with 256 x 256)
+//           gathering, they want waves (76 x 76 128 -> 256 3x3 of 64 images: 0.290 ms against 0.347 with 64 x 64; with 128 x 128 and 256 x 256
+//           1.1 and 1.9 times the time; 19 x 19 512 -> 1024 3x3 of 8 images 29.8 us with 64 x 64, 33.5 with 64 x 128)
 template <int TYPE, bool CONV, bool BYTES>
 static int launch_by_size(const MxProductArgs &a, hipStream_t s, char *name, size_t name_len)
 {
@@ -498,7 +502,9 @@ static int launch_by_size(const MxProductArgs &a, hipStream_t s, char *name, siz
     int t = 11;
     if (!rare) {
         if (CONV) t = grid(1, 2) >= 2 * cus ? 12 : 11;
-        else t = grid(4, 4) >= cus && a.kb >= 64 ? 44 : grid(2, 2) >= 2 * cus ? 22 : grid(1, 2) >= cus ? 12 : 11;
+        else if (grid(4, 4) >= cus && a.kb >= 64) t = 44;
+        else if (grid(2, 2) >= (a.kb >= 64 ? cus : 2 * cus)) t = 22;
+        else if (grid(1, 2) >= cus) t = 12;
     }
     if (name) snprintf(name, name_len, "mx_product<%dx%d>", t / 10 * 64, t % 10 * 64);
     if (rare) return launch_tile<TYPE, CONV, BYTES, true, 1, 1>(a, s);
