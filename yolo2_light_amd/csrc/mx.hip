@@ -24,17 +24,15 @@ struct DeviceScope {
     bool changed = false;
     int enter(const char *entry, int device)
     {
+        if (hipGetDevice(&before) == hipSuccess && before == device) return YL_OK;
         int count = 0;
         if (hipGetDeviceCount(&count) != hipSuccess || count <= 0) {
             set_error(std::string(entry) + ": no HIP device visible (libyolo2hip has no CPU fallback)");
             return YL_ERR_DEVICE;
         }
         if (device < 0 || device >= count) return refuse(entry, "no device " + std::to_string(device));
-        hipError_t e = hipGetDevice(&before);
-        if (e == hipSuccess && before != device) {
-            e = hipSetDevice(device);
-            changed = e == hipSuccess;
-        }
+        const hipError_t e = hipSetDevice(device);
+        changed = e == hipSuccess;
         if (e != hipSuccess) {
             set_error(std::string(entry) + ": " + hipGetErrorString(e));
             return YL_ERR_DEVICE;

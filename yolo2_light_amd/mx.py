@@ -11,6 +11,7 @@ tensor that requires a gradient raises.  Plumbing only: all arithmetic happens i
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional
 
 import torch
@@ -49,6 +50,11 @@ def _type(t, name: str) -> int:
 
 def _blocks(k: int) -> int:
     return (k + 4 * BLOCK - 1) // (4 * BLOCK) * 4          # yl_mx_blocks
+
+
+@functools.lru_cache(maxsize=None)
+def _gpu(index: int):
+    return torch.device("cuda", index)                     # an index takes torch longer than the device itself
 
 
 # the current stream of a device as a number; the public way makes an object of it first, which takes longer than a launch
@@ -115,20 +121,19 @@ def _matrix(m, name: str, device: Optional[int] = None) -> int:
 
 def _rows_of(x, name: str) -> Dense:
     """[..., k] as rows of k: the leading axes have to be one run of equal steps."""
-    kind = _type(x, name)
-    if x.dim() == 0:
+    kind, shape = _type(x, name), x.shape
+    if len(shape) == 2:
+        step, by = x.stride()
+        return Dense(x.data_ptr(), kind, 1, shape[0], shape[1], 0, step, by)
+    if len(shape) == 0:
         _fail("%s has no axis" % name)
-    if x.dim() == 2:
-        rows, step = x.shape[0], x.stride(0)
-    elif x.dim() == 1:
-        rows, step = 1, 0
-    else:
-        try:
-            flat = x.view(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1])
-        except RuntimeError:
-            _fail("the leading axes of %s cannot be taken as one axis of rows: make it contiguous" % name)
-        rows, step = flat.shape[0], flat.stride(0)
-    return Dense(x.data_ptr(), kind, 1, rows, x.shape[-1], 0, step, x.stride(-1))
+    if len(shape) == 1:
+        return Dense(x.data_ptr(), kind, 1, 1, shape[0], 0, 0, x.stride(0))
+    try:
+        flat = x.view(-1, shape[-1]) if x.numel() else x.reshape(0, shape[-1])
+    except RuntimeError:
+        _fail("the leading axes of %s cannot be taken as one axis of rows: make it contiguous" % name)
+    return Dense(x.data_ptr(), kind, 1, flat.shape[0], shape[-1], 0, flat.stride(0), x.stride(-1))
 
 
 def _map_of(x, name: str) -> Dense:
@@ -144,7 +149,7 @@ def _map_of(x, name: str) -> Dense:
 
 def _quantize(src: Dense, device: int, out: Optional[Matrix]) -> Matrix:
     if out is None:
-        out = Matrix.empty(src.batch * src.rows, src.k, device)
+        out = Matrix.empty(src.batch * src.rows, src.k, _gpu(device))
     else:
         _matrix(out, "out", device)
     check(lib.yl_mx_quantize(device, _stream(device), _ref(src), _ref(out._c)), "yl_mx_quantize")
@@ -183,7 +188,7 @@ def dequantize(q: Matrix, dtype=torch.float32, out=None):
     """The values of q, [rows, k]."""
     device = _matrix(q, "q")
     if out is None:
-        out = torch.empty(q.rows, q.k, dtype=dtype, device=device)
+        out = torch.empty((q.rows, q.k), dtype=dtype, device=_gpu(device))
     else:
         _tensor(out, "out", device)
     return _dequantize(q, out, _rows_of(out, "out"))
@@ -193,38 +198,42 @@ def dequantize_nchw(q: Matrix, batch: int, h: int, w: int, dtype=torch.float32, 
     """The values of a quantised map, [batch, q.k, h, w]."""
     device = _matrix(q, "q")
     if out is None:
-        out = torch.empty(batch, q.k, h, w, dtype=dtype, device=device)
+        out = torch.empty((batch, q.k, h, w), dtype=dtype, device=_gpu(device))
     else:
         _tensor(out, "out", device)
     return _dequantize(q, out, _map_of(out, "out"))
 
 
 def _epilogue(n: int, device: int, bias, activation, residual) -> Optional[MxEpilogue]:
-    act = ACTIVATIONS.get(activation) if isinstance(activation, str) else activation
-    if act is None or not isinstance(act, int):
+    act = ACTIVATIONS.get(activation, activation)
+    if not isinstance(act, int):
         _fail("unknown activation %r" % (activation,))
+    if bias is None and residual is None and act == 3:
+        return None
     b = r = None
     if bias is not None:
         _tensor(bias, "bias", device)
-        if bias.dtype is not torch.float32 or bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous():
+        if bias.dtype is not torch.float32 or bias.shape != (n,) or not bias.is_contiguous():
             _fail("bias is a contiguous float32 tensor of %d values" % n)
         b = bias.data_ptr()
     if residual is not None:
         r = residual.data_ptr()
-    elif b is None and act == 3:
-        return None
     return MxEpilogue(b, act, r, residual.stride(0) if r is not None else 0)
 
 
 def _linear_args(lead, m: int, w: Matrix, device: int, bias, activation, residual, dtype, out):
     n = w.rows
     if out is None:
-        out = torch.empty((*lead, n), dtype=dtype, device=device)
+        kind = _TYPES.get(dtype)
+        if kind is None:
+            _fail("dtype is %s: float32, float16 and bfloat16 are made" % dtype)
+        out = torch.empty((*lead, n), dtype=dtype, device=_gpu(device))
+        y = Dense(out.data_ptr(), kind, 1, m, n, 0, n, 1)
     else:
         _tensor(out, "out", device)
         if tuple(out.shape) != (*lead, n):
             _fail("out is not %s" % ((*lead, n),))
-    y = _rows_of(out, "out")
+        y = _rows_of(out, "out")
     if residual is not None:
         _tensor(residual, "residual", device)
         if residual.dtype is not out.dtype or residual.shape != out.shape:
@@ -257,7 +266,7 @@ def linear(x, w: Matrix, bias=None, activation="linear", residual=None, dtype=No
     m = xd.rows
     out, y, e = _linear_args(x.shape[:-1], m, w, device, bias, activation, residual, dtype or x.dtype, out)
     need = lib.yl_mx_linear_workspace(m, xd.k)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=_gpu(device)) if need else None
     check(lib.yl_mx_linear(device, _stream(device), _ref(xd), _ref(w._c), None if e is None else _ref(e), _ref(y),
                            ws.data_ptr() if need else None, need), "yl_mx_linear")
     return out
@@ -282,12 +291,12 @@ def conv2d(x: Matrix, filters: Matrix, batch: int, h: int, w: int, size: int, st
         if out is not None:
             _fail("out is given, but want is \"mx\"")
     elif out is None:
-        out = torch.empty(batch, n, oh, ow, dtype=torch.float32, device=device)
+        out = torch.empty((batch, n, oh, ow), dtype=torch.float32, device=_gpu(device))
     else:
         _tensor(out, "out", device)
         if out.dtype is not torch.float32 or out.shape != (batch, n, oh, ow) or not out.is_contiguous():
             _fail("out is a contiguous float32 tensor of the result's shape")
-    q = Matrix.empty(batch * oh * ow, n, device) if want != "float" else None
+    q = Matrix.empty(batch * oh * ow, n, _gpu(device)) if want != "float" else None
     e = _epilogue(n, device, bias, activation, residual)
     shape = MxConv(batch, h, w, size, stride, pad)
     check(lib.yl_mx_conv2d(device, _stream(device), _ref(x._c), _ref(filters._c), _ref(shape), None if e is None else _ref(e),
