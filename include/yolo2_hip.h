@@ -499,7 +499,8 @@ typedef struct yl_dense {
 typedef struct yl_mx_epilogue {
     const float *bias;          /* one a column of w / filter, or NULL */
     int activation;             /* YL_LINEAR, YL_LEAKY, ... (any activation of this header) */
-    const void *residual;       /* y's type and shape, or NULL; may be y itself, may not otherwise overlap it */
+    const void *residual;       /* y's type and shape, or NULL; may be y itself or lie beside it in the same rows, may not
+                                   otherwise overlap it */
     int64_t residual_stride;    /* elements from row to row (the convolution: ignored, y's layout) */
 } yl_mx_epilogue;
 
@@ -515,7 +516,7 @@ int yl_mx_quantize(int device, void *stream, const yl_dense *src, const yl_mx_ma
 int yl_mx_dequantize(int device, void *stream, const yl_mx_matrix *src, const yl_dense *dst);
 
 /* y[m][n] = activate(sum over k of x[m][k] * w[n][k] + bias[n]) + residual[m][n], summed in 32 bits.
- * y: batch 1, rows = x->rows, k = w->rows, k_stride 1; it may not overlap the operands. */
+ * y: batch 1, rows = x->rows, k = w->rows, k_stride 1; it may not overlap the operands (beside them in the same rows is well). */
 int yl_mx_matmul(int device, void *stream, const yl_mx_matrix *x, const yl_mx_matrix *w, const yl_mx_epilogue *epilogue, const yl_dense *y);
 
 /* yl_mx_matmul on yl_mx_quantize(x), the same bits, in one call.  x: batch 1.  `workspace` is device memory of at least
@@ -530,7 +531,7 @@ int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix
  * filters->k = size * size * ceil(channels / 32) * 32.
  * out (float [batch][filters][oh][ow], NULL if not wanted) = activate(convolution + bias) + residual (the same layout);
  * q_out (NULL if not wanted): the same values rounded to MXFP4 as the next layer's x, rows = batch * oh * ow, k = filters.
- * oh = (h + 2 * pad - size) / stride + 1, ow likewise; size <= 5. */
+ * oh = (h + 2 * pad - size) / stride + 1, ow likewise; size <= 5, pad < size, channels <= 2^18, an image's result below 2 GB. */
 typedef struct yl_mx_conv {
     int batch, h, w, size, stride, pad;
 } yl_mx_conv;

@@ -237,6 +237,20 @@ def test_strided_results_and_residuals(mx, m, n, k, dtype):
     close(mx.matmul(x, w, residual=one, dtype=TYPES[dtype]), want, tol)
 
 
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_operands_and_results_side_by_side(mx, m):
+    """x, the residual and the result as columns of one buffer."""
+    n, k = 72, 96
+    w, _ = make(mx, n, k, 1)
+    x, res = rand(m, k, seed=2), rand(m, n, seed=3)
+    want = mx.linear(x.cuda(), w, residual=res.cuda())
+    buf = torch.full((m, k + 2 * n + 8), 5.0, device="cuda")
+    buf[:, :k], buf[:, k:k + n] = x.cuda(), res.cuda()
+    mx.linear(buf[:, :k], w, residual=buf[:, k:k + n], out=buf[:, k + n:k + 2 * n])
+    assert torch.equal(buf[:, k + n:k + 2 * n], want) and (buf[:, k + 2 * n:] == 5).all()
+    assert torch.equal(buf[:, :k].cpu(), x) and torch.equal(buf[:, k:k + n].cpu(), res)
+
+
 @pytest.mark.parametrize("ld", [3, 5, 6, 7, 9])
 @pytest.mark.parametrize("m", [1, 20, 150])
 def test_rows_of_any_stride(mx, ld, m):

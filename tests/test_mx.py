@@ -147,7 +147,12 @@ def test_refused_products():
                     (MxEpilogue(96 * MB, 3, None, 0), "bias"), (MxEpilogue(None, 3, 96 * MB + 4, 8), "residual"), (MxEpilogue(None, 3, 96 * MB, 16), "residual"),
                     (MxEpilogue(None, 3, 200 * MB, -1), "residual"), (MxEpilogue(None, 3, 200 * MB + 2, 8), "residual")):
         refused(matmul(e=e), what)
+    beside = {**Y, "rs": 16}
+    refused(matmul(y=beside, e=MxEpilogue(None, 3, 96 * MB + 7 * 4, 16)), "residual")          # one column in common
+    refused(matmul(y=beside, e=MxEpilogue(None, 3, 96 * MB + 9 * 4, 16)), "residual")          # and around the end of a row
     if not HAVE_GPU:
+        accepted(matmul(y=beside, e=MxEpilogue(None, 3, 96 * MB + 8 * 4, 16)))                 # beside it in the same rows
+        accepted(matmul(y={**beside, "data": 96 * MB + 8 * 4}, e=MxEpilogue(None, 3, 96 * MB, 16)))
         accepted(matmul(e=MxEpilogue(None, 3, 96 * MB, 8)))            # the residual may be y itself
         accepted(matmul(e=MxEpilogue(128 * MB, 7, 200 * MB, 8)))
         accepted(matmul(x={**X, "rows": 0, "codes": None, "scales": None}, y={**Y, "rows": 0, "data": None}))
@@ -166,7 +171,9 @@ def test_refused_linear_layers():
         refused(linear(x=dense(**big), y=wide, ws=at * MB), "overlaps")
     refused(linear(x=dense(**big), y=wide, e=MxEpilogue(112 * MB, 3, None, 0)), "overlaps")
     refused(linear(x=dense(**big), y=wide, e=MxEpilogue(None, 3, 112 * MB, 8)), "overlaps")
+    refused(linear(x=dense(rs=80), y={**Y, "data": 48 * MB + 63 * 4, "rs": 80}), "overlaps x")
     if not HAVE_GPU:
+        accepted(linear(x=dense(rs=80), y={**Y, "data": 48 * MB + 64 * 4, "rs": 80}))          # behind x in the same rows
         accepted(linear())
         accepted(linear(x=dense(**big), y=wide))
 

@@ -12,10 +12,14 @@ namespace {
 constexpr int64_t MX_MAX_ELEMENTS = (int64_t)1 << 46;     // what a stride or a size may address: products of two stay in 64 bits
 constexpr int64_t MX_MAX_LD = (int64_t)1 << 19;           // blocks a row: 32-bit offsets inside a tile of 256 rows
 
-int refuse(const char *entry, const std::string &what)
+// nothing may be thrown through a C entry: an error text that finds no memory is left out
+int refuse(const char *entry, const char *what, int rc = YL_ERR_ARG) noexcept
 {
-    set_error(std::string(entry) + ": " + what);
-    return YL_ERR_ARG;
+    try {
+        set_error(std::string(entry) + ": " + what);
+    } catch (...) {
+    }
+    return rc;
 }
 
 // the caller's current device is the same after the call
@@ -27,26 +31,19 @@ struct DeviceScope {
         if (hipGetDevice(&before) == hipSuccess && before == device) return YL_OK;
         int count = 0;
         if (hipGetDeviceCount(&count) != hipSuccess || count <= 0) {
-            set_error(std::string(entry) + ": no HIP device visible (libyolo2hip has no CPU fallback)");
-            return YL_ERR_DEVICE;
+            return refuse(entry, "no HIP device visible (libyolo2hip has no CPU fallback)", YL_ERR_DEVICE);
         }
-        if (device < 0 || device >= count) return refuse(entry, "no device " + std::to_string(device));
+        if (device < 0 || device >= count) return refuse(entry, "no such device");
         const hipError_t e = hipSetDevice(device);
         changed = e == hipSuccess;
-        if (e != hipSuccess) {
-            set_error(std::string(entry) + ": " + hipGetErrorString(e));
-            return YL_ERR_DEVICE;
-        }
-        return YL_OK;
+        return e == hipSuccess ? YL_OK : refuse(entry, hipGetErrorString(e), YL_ERR_DEVICE);
     }
     ~DeviceScope() { if (changed) (void)hipSetDevice(before); }
 };
 
 int launched(const char *entry, int e)
 {
-    if (e == 0) return YL_OK;
-    set_error(std::string(entry) + ": " + hipGetErrorString((hipError_t)e));
-    return YL_ERR_DEVICE;
+    return e == 0 ? YL_OK : refuse(entry, hipGetErrorString((hipError_t)e), YL_ERR_DEVICE);
 }
 
 int64_t blocks_of(int64_t k) { return (k + MX_BLOCK - 1) / MX_BLOCK; }
@@ -57,6 +54,15 @@ struct Range {
     bool meets(const Range &o) const { return from < o.to && o.from < to; }
 };
 Range range_of(const void *p, int64_t bytes) { return {(uintptr_t)p, (uintptr_t)p + (uintptr_t)(bytes > 0 ? bytes : 0)}; }
+
+// Two sets of rows of one buffer side by side: the same row stride, and the column windows of `n` and `m` bytes do not meet.
+bool beside(const void *a, int64_t n, const void *b, int64_t m, int64_t stride)
+{
+    if (stride <= 0) return false;
+    int64_t d = (int64_t)((uintptr_t)b - (uintptr_t)a) % stride;
+    if (d < 0) d += stride;
+    return d >= n && d + m <= stride;
+}
 
 const char *check_matrix(const yl_mx_matrix *m)
 {
@@ -140,7 +146,9 @@ const char *check_product(int64_t x_rows, int64_t x_k, const yl_mx_matrix *w, co
         if (e->residual_stride < 0 || e->residual_stride > MX_MAX_ELEMENTS || (y->rows > 1 && e->residual_stride > MX_MAX_ELEMENTS / (y->rows - 1))) return "residual_stride is negative or too large";
         const Range r = range_of(e->residual, ((y->rows - 1) * e->residual_stride + y->k) * type_bytes(y->type));
         const bool same = e->residual == y->data && (y->rows <= 1 || e->residual_stride == y->row_stride);
-        if (!same && out.meets(r)) return "y overlaps the residual";
+        const int64_t el = type_bytes(y->type);
+        const bool apart = e->residual_stride == y->row_stride && beside(y->data, y->k * el, e->residual, y->k * el, y->row_stride * el);
+        if (!same && !apart && out.meets(r)) return "y overlaps the residual";
     }
     a->b_codes = w->codes; a->b_scales = w->scales; a->b_ld = w->ld;
     a->I = x_rows; a->J = w->rows; a->k = w->k; a->kb = blocks_of(w->k);
@@ -221,7 +229,9 @@ int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix
     if (x->batch != 1) return refuse(entry, "x has more than one batch");
     if (const char *m = check_product(x->rows, x->k, w, epilogue, y, &a)) return refuse(entry, m);
     const Range in = dense_range(x), out = dense_range(y);
-    if (out.meets(in)) return refuse(entry, "y overlaps x");
+    const int64_t xe = type_bytes(x->type), ye = type_bytes(y->type);
+    const bool apart = x->k_stride == 1 && x->row_stride * xe == y->row_stride * ye && beside(x->data, x->k * xe, y->data, y->k * ye, y->row_stride * ye);
+    if (!apart && out.meets(in)) return refuse(entry, "y overlaps x");
     const int64_t need = yl_mx_linear_workspace(x->rows, x->k);
     if (need > 0) {
         if (!workspace || workspace_bytes < need) return refuse(entry, "workspace is smaller than yl_mx_linear_workspace(x->rows, x->k)");

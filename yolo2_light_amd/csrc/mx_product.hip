@@ -134,15 +134,16 @@ template <bool RARE>
 __device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const mx_f32x16 &acc, int ib, int64_t j, bool ok, int half,
                                                  __amdgpu_buffer_rsrc_t out, __amdgpu_buffer_rsrc_t residual, int at)
 {
-    const int I = (int)p.I, plane = p.OH * p.OW * 4;
+    const int I = (int)p.I;
+    const unsigned plane = (unsigned)p.OH * (unsigned)p.OW * 4u;      // bytes; a whole image's planes are below 2^32
     float y[16], add[16];
     int off[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const int r = 8 * (e / 4) + e % 4;                 // + 4 half, in the lane's offset
-        off[e] = ok && ib + r + 4 * half < I ? at + 4 * half * plane : -1;
+        off[e] = ok && ib + r + 4 * half < I ? (int)((unsigned)at + 4u * half * plane) : -1;
         add[e] = 0.f;
-        if (p.residual) add[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(residual, off[e], (ib + r) * plane, 0));
+        if (p.residual) add[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(residual, off[e], (int)((ib + r) * plane), 0));
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -155,7 +156,7 @@ __device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const m
     if (p.out) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y[e]), out, off[e], (ib + 8 * (e / 4) + e % 4) * plane, 0);
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y[e]), out, off[e], (int)((ib + 8 * (e / 4) + e % 4) * plane), 0);
     }
     if (p.q_codes) {
 #pragma unroll
