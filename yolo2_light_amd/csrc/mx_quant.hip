@@ -6,6 +6,9 @@
 //            taken across the four, each makes the 32 bits of its own codes, so a wave reads and writes contiguous memory
 //   columns  any other strides, in practice NCHW maps, where rows (pixels) are contiguous: a lane holds a whole block of one row, so a
 //            wave reads 64 neighbouring pixels of a channel at a time; codes go through LDS, so that a row's blocks leave together
+// MI355X: 16 x 256 x 76 x 76 FP32 to MXFP4 and back 20.0 + 20.3 us, 6.0 TB/s (out of the 256 MB cache; 51 us from HBM, where a large copy
+// makes 5.1 TB/s); 4096 x 4096 BF16 rows 10.1 us; one row of 4096 2.3 us, which is a launch.  One thread a block with scalar loads, the
+// first form, took 52 us for the map's pair and 27 instead of 8.4 us for the pair on 3001 x 1005 FP16 values in rows of 1016.
 #include "mx_device.h"
 #include "mx.h"
 
