@@ -210,6 +210,13 @@ def test_refused_convolutions():
         accepted(conv(x=matrix(rows=0, k=32, ld=1), shape=(0, 4, 4, 3, 1, 1)))
 
 
+def test_as_many_rows_as_32_bits_count():
+    most = 0x7fffffff - 256
+    for x, y in ((dict(rows=most + 1, k=32, ld=1), dict(rows=most + 1, k=1, data=1 << 50)), (dict(rows=1, k=32, ld=1), dict(rows=1, k=most + 1, data=1 << 50))):
+        w = dict(rows=y["k"], k=32, ld=1, codes=1 << 45, scales=1 << 47)
+        refused(matmul(x={**x, "codes": 1 << 40, "scales": 1 << 43}, w=w, y=y), "2^31 - 257")
+
+
 def test_no_such_device():
     for device in (-1, 4096):
         rc = quantize(dense(), matrix(), device=device)

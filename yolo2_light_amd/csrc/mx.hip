@@ -12,6 +12,8 @@ namespace {
 constexpr int64_t MX_MAX_ELEMENTS = (int64_t)1 << 46;     // what a stride or a size may address: products of two stay in 64 bits
 constexpr int64_t MX_MAX_LD = (int64_t)1 << 19;           // blocks a row: 32-bit offsets inside a tile of 256 rows
 
+constexpr int64_t MX_MAX_ROWS = 0x7fffffff - 256;         // rows of a product's side: the end of a tile of 256 is still a 32-bit number
+
 // nothing may be thrown through a C entry: an error text that finds no memory is left out
 int refuse(const char *entry, const char *what, int rc = YL_ERR_ARG) noexcept
 {
@@ -137,7 +139,7 @@ const char *check_product(int64_t x_rows, int64_t x_k, const yl_mx_matrix *w, co
     if (y->batch != 1 || y->rows != x_rows || y->k != w->rows) return "y is not one batch of x's rows by w's rows";
     if (y->k > 1 && y->k_stride != 1) return "y's k_stride is not 1";
     if (y->rows > 1 && y->row_stride < y->k) return "rows of y overlap";
-    if (x_rows > 0x7fffffff || w->rows > 0x7fffffff) return "more than 2^31 - 1 rows";
+    if (x_rows > MX_MAX_ROWS || w->rows > MX_MAX_ROWS) return "more than 2^31 - 257 rows";
     const Range out = dense_range(y);
     if (out.meets(codes_range(w)) || out.meets(scales_range(w))) return "y overlaps w";
     if (e && e->bias && out.meets(range_of(e->bias, w->rows * 4))) return "y overlaps the bias";
@@ -271,7 +273,7 @@ int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
     if (oh_num < 0 || ow_num < 0) return refuse(entry, "the filter is larger than the padded map");
     const int oh = oh_num / c.stride + 1, ow = ow_num / c.stride + 1;
     const int64_t J = (int64_t)c.batch * oh * ow, I = filters->rows;
-    if (J > 0x7fffffff || I > 0x7fffffff || x->rows > 0x7fffffff || (J > 0 && I > MX_MAX_ELEMENTS / J)) return refuse(entry, "map or result is too large");
+    if (J > MX_MAX_ROWS || I > MX_MAX_ROWS || x->rows > MX_MAX_ROWS || (J > 0 && I > MX_MAX_ELEMENTS / J)) return refuse(entry, "map or result is too large");
     // the kernels' 32-bit offsets: the rows of the map under 256 neighbouring positions of the result
     const int64_t area = (int64_t)oh * ow, part = 256 % area;
     const int64_t reach = (256 / area + 1) * c.h * c.w + ((part + ow - 1) / ow + 1) * c.stride * c.w + (int64_t)(c.size + 1) * (c.w + 1);

@@ -11,6 +11,7 @@
 // first form, took 52 us for the map's pair and 27 instead of 8.4 us for the pair on 3001 x 1005 FP16 values in rows of 1016.
 #include "mx_device.h"
 #include "mx.h"
+#include "kernels.h"
 
 namespace yl {
 
@@ -74,23 +75,23 @@ __global__ __launch_bounds__(256) void mx_dequantize_rows_kernel(const unsigned 
     }
 }
 
-// A workgroup takes 64 rows by 8 blocks, a wave two of the blocks.
-constexpr int MX_COLS_ROWS = 64, MX_COLS_BLOCKS = 8;
+// A workgroup takes 64 rows by BLOCKS blocks: 8, two a wave, or 4 where 8 would leave CUs without work.
+constexpr int MX_COLS_ROWS = 64;
 
-template <int TYPE>
+template <int TYPE, int BLOCKS>
 __global__ __launch_bounds__(256) void mx_quantize_columns_kernel(MxDense s, uint4 *__restrict__ codes, unsigned char *__restrict__ scales, int64_t ld, int64_t kb, int64_t groups)
 {
-    __shared__ uint4 lc[MX_COLS_ROWS * MX_COLS_BLOCKS];
-    __shared__ unsigned char ls[MX_COLS_ROWS * MX_COLS_BLOCKS];
+    __shared__ uint4 lc[MX_COLS_ROWS * BLOCKS];
+    __shared__ unsigned char ls[MX_COLS_ROWS * BLOCKS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tile = blockIdx.x / groups, j0 = (blockIdx.x - tile * groups) * MX_COLS_BLOCKS;
+    const int64_t tile = blockIdx.x / groups, j0 = (blockIdx.x - tile * groups) * BLOCKS;
     const int64_t row0 = tile * MX_COLS_ROWS, rows = s.batch * s.rows, row = row0 + lane;
-    const int blocks = (int)min((int64_t)MX_COLS_BLOCKS, kb - j0), count = (int)min((int64_t)MX_COLS_ROWS, rows - row0);
+    const int blocks = (int)min((int64_t)BLOCKS, kb - j0), count = (int)min((int64_t)MX_COLS_ROWS, rows - row0);
     if (lane < count) {
         const int64_t b = s.batch > 1 ? row / s.rows : 0;
         const int64_t at = b * s.batch_stride + (row - b * s.rows) * s.row_stride;
 #pragma unroll
-        for (int h = 0; h < MX_COLS_BLOCKS / 4; ++h) {
+        for (int h = 0; h < BLOCKS / 4; ++h) {
             const int j = wave + 4 * h;
             if (j >= blocks) break;
             const int64_t k0 = (j0 + j) * MX_BLOCK;
@@ -121,16 +122,16 @@ __global__ __launch_bounds__(256) void mx_quantize_columns_kernel(MxDense s, uin
     }
 }
 
-template <int TYPE>
+template <int TYPE, int BLOCKS>
 __global__ __launch_bounds__(256) void mx_dequantize_columns_kernel(const uint4 *__restrict__ codes, const unsigned char *__restrict__ scales, int64_t ld, MxDense d, int64_t kb, int64_t groups)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t tile = blockIdx.x / groups, j0 = (blockIdx.x - tile * groups) * MX_COLS_BLOCKS;
+    const int64_t tile = blockIdx.x / groups, j0 = (blockIdx.x - tile * groups) * BLOCKS;
     const int64_t row = tile * MX_COLS_ROWS + lane;
     if (row >= d.batch * d.rows) return;
     const int64_t b = d.batch > 1 ? row / d.rows : 0;
     const int64_t at = b * d.batch_stride + (row - b * d.rows) * d.row_stride;
-    for (int64_t j = j0 + wave; j < kb && j < j0 + MX_COLS_BLOCKS; j += 4) {
+    for (int64_t j = j0 + wave; j < kb && j < j0 + BLOCKS; j += 4) {
         const uint4 q = codes[row * ld + j];
         const unsigned byte = scales[row * ld + j];
         const unsigned w[4] = {q.x, q.y, q.z, q.w};
@@ -147,6 +148,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_columns_kernel(const uint4 
     }
 }
 
+static int columns_blocks(int64_t tiles, int64_t kb) { return tiles * ((kb + 7) / 8) >= 2 * (int64_t)device_cu_count() ? 8 : 4; }
+
 template <int TYPE>
 static int launch_quantize(const MxDense &src, void *codes, void *scales, int64_t ld, hipStream_t s)
 {
@@ -157,9 +160,12 @@ static int launch_quantize(const MxDense &src, void *codes, void *scales, int64_
         if (n < 0x60000000) hipLaunchKernelGGL((mx_quantize_rows_kernel<TYPE, unsigned>), grid, dim3(256), 0, s, src, (unsigned *)codes, (unsigned char *)scales, ld, (unsigned)kb, (unsigned)n);
         else hipLaunchKernelGGL((mx_quantize_rows_kernel<TYPE, int64_t>), grid, dim3(256), 0, s, src, (unsigned *)codes, (unsigned char *)scales, ld, kb, n);
     } else {
-        const int64_t groups = (kb + MX_COLS_BLOCKS - 1) / MX_COLS_BLOCKS, g = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS * groups;
+        const int64_t tiles = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS;
+        const int blocks = columns_blocks(tiles, kb);
+        const int64_t groups = (kb + blocks - 1) / blocks, g = tiles * groups;
         if (g > 0x7fffffff) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL((mx_quantize_columns_kernel<TYPE>), dim3((unsigned)g), dim3(256), 0, s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
+        if (blocks == 8) hipLaunchKernelGGL((mx_quantize_columns_kernel<TYPE, 8>), dim3((unsigned)g), dim3(256), 0, s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
+        else hipLaunchKernelGGL((mx_quantize_columns_kernel<TYPE, 4>), dim3((unsigned)g), dim3(256), 0, s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
     }
     return (int)hipGetLastError();
 }
@@ -174,9 +180,12 @@ static int launch_dequantize(const void *codes, const void *scales, int64_t ld, 
         if (n < 0x60000000) hipLaunchKernelGGL((mx_dequantize_rows_kernel<TYPE, unsigned>), grid, dim3(256), 0, s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, (unsigned)kb, (unsigned)n);
         else hipLaunchKernelGGL((mx_dequantize_rows_kernel<TYPE, int64_t>), grid, dim3(256), 0, s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, kb, n);
     } else {
-        const int64_t groups = (kb + MX_COLS_BLOCKS - 1) / MX_COLS_BLOCKS, g = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS * groups;
+        const int64_t tiles = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS;
+        const int blocks = columns_blocks(tiles, kb);
+        const int64_t groups = (kb + blocks - 1) / blocks, g = tiles * groups;
         if (g > 0x7fffffff) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL((mx_dequantize_columns_kernel<TYPE>), dim3((unsigned)g), dim3(256), 0, s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
+        if (blocks == 8) hipLaunchKernelGGL((mx_dequantize_columns_kernel<TYPE, 8>), dim3((unsigned)g), dim3(256), 0, s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
+        else hipLaunchKernelGGL((mx_dequantize_columns_kernel<TYPE, 4>), dim3((unsigned)g), dim3(256), 0, s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
     }
     return (int)hipGetLastError();
 }
