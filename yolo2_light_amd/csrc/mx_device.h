@@ -5,6 +5,7 @@
 #include <hip/hip_fp16.h>
 
 #include "../../include/yolo2_hip.h"
+#include "activations.h"
 
 namespace yl {
 
@@ -68,6 +69,15 @@ template <int TYPE>
 __device__ __forceinline__ mx_u32x4 mx_load_vec(const void *p, int64_t i) { return *reinterpret_cast<const mx_u32x4 *>(reinterpret_cast<const char *>(p) + i * (16 / MX_VEC<TYPE>)); }
 template <int TYPE>
 __device__ __forceinline__ void mx_store_vec(void *p, int64_t i, mx_u32x4 v) { *reinterpret_cast<mx_u32x4 *>(reinterpret_cast<char *>(p) + i * (16 / MX_VEC<TYPE>)) = v; }
+
+// activate(): LINEAR, LEAKY and RELU (x * (x > 0)) by one slope below zero, in 32 bits; the others only where RARE says so
+template <bool RARE>
+__device__ __forceinline__ float mx_activate(float v, int act)
+{
+    if (RARE && act != YL_LINEAR && act != YL_LEAKY && act != YL_RELU) return yl_activate(v, act);
+    const float slope = act == YL_LINEAR ? 1.f : act == YL_LEAKY ? .1f : 0.f;
+    return v > 0.f ? v : __fmul_rn(v, slope);
+}
 
 // The scale byte of a block whose largest magnitude has the FP32 bits `top` (exponent field f): floor(log2) is f - 127, the largest
 // E2M1 exponent is 2, so the byte is f - 2, not below 0 (2^-127; subnormals and zero have f = 0).  f = 255 is an Inf or a NaN.

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(MX_FEW_THREADS) void mx_product_few_kernel(MxProduc
 #pragma unroll
         for (int w = 1; w < MX_FEW_WAVES; ++w) v += sums[w * C * C + t];
         if (p.bias) v += p.bias[jj];
-        v = yl_act_epilogue(v, p.act);
+        v = mx_activate<true>(v, p.act);
         if (p.residual) v += mx_load<TYPE>(p.residual, (int64_t)i * p.residual_stride + jj);
         mx_store<TYPE>(p.out, (int64_t)i * p.out_stride + jj, v);
     }

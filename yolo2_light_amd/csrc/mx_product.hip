@@ -37,14 +37,6 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_v4i a, mx_v4i b, mx_f32x16 c, in
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a), mx_operand(b), c, 4, 4, S, sa, S, sb);
 }
 
-// LINEAR, LEAKY and RELU in line (activations.h's arithmetic); the others only where RARE says so
-template <bool RARE>
-__device__ __forceinline__ float mx_activate(float v, int act)
-{
-    if constexpr (RARE) return yl_act_epilogue(v, act);
-    else return v > 0.f || act == YL_LINEAR ? v : act == YL_LEAKY ? (float)(.1 * (double)v) : __fmul_rn(v, 0.f);
-}
-
 // A strip of D, 32 rows from ib by COLS columns from jb, in LDS: + bias, activation, + residual, to rows of memory.  In 16-byte vectors
 // where every row's begin on one, else by single values; AHEAD rows' addends are requested before the first is used.
 template <int TYPE, bool RARE, bool WIDE, int COLS, int PITCH>
@@ -134,38 +126,40 @@ __device__ __forceinline__ void mx_side_block(const MxProductArgs &p, int64_t j,
 }
 
 // A convolution's 32 x 32 tile of D from registers to planes of memory.  `at`: byte offset of (this lane's position, row 0 of the image's
-// planes) in `out`, -1 where there is no such position.
-template <bool RARE>
-__device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const mx_f32x16 &acc, int ib, int64_t j, bool ok, int half,
+// planes) in `out`; WHOLE: all 32 rows are filters.  This and the index arithmetic in front of the panels are most of a layer with few
+// channels: the bias comes as four vectors, rows are offsets of the instruction (76 x 76 256 -> 128 1x1 of 8 images 16.4 -> 10 us).
+template <bool RARE, bool WHOLE>
+__device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const mx_f32x16 &acc, int ib, int64_t j, bool ok, int half, __amdgpu_buffer_rsrc_t bias,
                                                  __amdgpu_buffer_rsrc_t out, __amdgpu_buffer_rsrc_t residual, int at)
 {
     const int I = (int)p.I;
     const unsigned plane = (unsigned)p.OH * (unsigned)p.OW * 4u;      // bytes; a whole image's planes are below 2^32
+    const int lane_off = ok ? (int)((unsigned)at + 4u * half * plane) : -1;
+    auto off = [&](int e) { return WHOLE || ib + 8 * (e / 4) + e % 4 + 4 * half < I ? lane_off : -1; };
+    auto row = [&](int e) { return (int)((ib + 8 * (e / 4) + e % 4) * plane); };
     float y[16], add[16];
-    int off[16];
+    mx_u32x4 b[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int r = 8 * (e / 4) + e % 4;                 // + 4 half, in the lane's offset
-        off[e] = ok && ib + r + 4 * half < I ? (int)((unsigned)at + 4u * half * plane) : -1;
-        add[e] = 0.f;
-        if (p.residual) add[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(residual, off[e], (int)((ib + r) * plane), 0));
+    for (int q = 0; q < 4; ++q) b[q] = __builtin_amdgcn_raw_buffer_load_b128(bias, 16 * half, (ib + 8 * q) * 4, 0);      // zeros where there is none
+    if (p.residual) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) add[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(residual, off(e), row(e), 0));
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        const int i = ib + 8 * (e / 4) + e % 4 + 4 * half;
-        float v = acc[e];
-        if (p.bias) v += p.bias[min(i, I - 1)];
-        y[e] = mx_activate<RARE>(v, p.act);
+        const unsigned w = b[e / 4][e % 4];
+        y[e] = mx_activate<RARE>(acc[e] + __builtin_bit_cast(float, w), p.act);
         if (p.residual) y[e] += add[e];
     }
     if (p.out) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y[e]), out, off[e], (int)((ib + 8 * (e / 4) + e % 4) * plane), 0);
+        for (int e = 0; e < 16; ++e) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y[e]), out, off(e), row(e), 0);
     }
     if (p.q_codes) {
+        if (!WHOLE) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = off[e] != -1 ? y[e] : 0.f;
+            for (int e = 0; e < 16; ++e) y[e] = ib + 8 * (e / 4) + e % 4 + 4 * half < I ? y[e] : 0.f;
+        }
         mx_side_block(p, j, ok, ib, half, y);
     }
 }
@@ -252,6 +246,7 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
         if (!CONV) return j - j0;
         const int image = d.area(j), pix = j - image * d.area.d, oy = d.width(pix), ox = pix - oy * p.OW;
         const int y = oy * p.stride - p.pad, x = ox * p.stride - p.pad;
+        if (p.size == 1) return ((image - cj_image) * p.H + y - cj_y) * p.W + x;      // pad < size: no tap is outside
         // columns of the filter from -x to W - x are inside, lines likewise
         const unsigned columns = ((1u << min(max(p.W - x, 0), p.size)) - 1u) & (~0u << max(-x, 0));
         unsigned in = 0;
@@ -380,7 +375,22 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
         __builtin_amdgcn_sched_barrier(0);                                                                                       \
     }
 
-    if (panels > 0) {
+    constexpr int MM = TI * TJ, HALF = ITEMS / 2, EARLY = MM / 2 > 0 ? MM / 2 : 1;
+    if (panels == 1) {                                     // nothing to overlap
+        begin_load(0);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) load(0, 0, k);
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) store(0, 0, k);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < READS; ++k) { fetch_scale(0, k); fetch(0, 0, 0, k); }
+        take_scales();
+        MX_STEP(0, 0, READS, EARLY, fetch(0, 1, 1, k);)
+        MX_STEP(1, 1, READS, EARLY, fetch(0, 2, 0, k);)
+        MX_STEP(2, 0, READS, EARLY, fetch(0, 3, 1, k);)
+        MX_STEP(3, 1, 0, EARLY, )
+    } else if (panels > 1) {
         begin_load(0);
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) load(0, 0, k);
@@ -399,7 +409,6 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
 #pragma unroll
         for (int k = 0; k < READS; ++k) { fetch(0, 0, 0, k); fetch_scale(0, k); }
         take_scales();
-        constexpr int MM = TI * TJ, HALF = ITEMS / 2, EARLY = MM / 2 > 0 ? MM / 2 : 1;
         // Panel PN while panel PN + 1 lies in set SET of the registers: it is stored, and panel PN + 1 + SETS requested in its place.  Panels
         // behind the last one read as zeros and nothing of memory (every offset is out of its descriptor's range), so the loop needs no
         // case for its end.
@@ -435,6 +444,7 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
         const int area = d.area.d, image0 = d.area(j0 + wj0);
         const int64_t planes = (int64_t)I * area * 4;
         const __amdgpu_buffer_rsrc_t out = resource(p.out ? p.out : p.a_codes, p.out ? image0 * planes : 0, p.out ? (p.batch - image0) * planes : 0);
+        const __amdgpu_buffer_rsrc_t bias = resource(p.bias ? (const void *)p.bias : p.a_codes, 0, p.bias ? (int64_t)I * 4 : 0);
         const __amdgpu_buffer_rsrc_t residual = resource(p.residual ? p.residual : p.a_codes, p.residual ? image0 * planes : 0, p.residual ? (p.batch - image0) * planes : 0);
 #pragma unroll
         for (int tj = 0; tj < TJ; ++tj) {
@@ -443,7 +453,8 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
 #pragma unroll
             for (int ti = 0; ti < TI; ++ti) {
                 const int ib = i0 + wi0 + ti * 32;
-                if (ib < I) mx_finish_planes<RARE>(p, acc[ti][tj], ib, j, j < J, half, out, residual, at);
+                if (ib + 32 <= I) mx_finish_planes<RARE, true>(p, acc[ti][tj], ib, j, j < J, half, bias, out, residual, at);
+                else if (ib < I) mx_finish_planes<RARE, false>(p, acc[ti][tj], ib, j, j < J, half, bias, out, residual, at);
                 __builtin_amdgcn_sched_barrier(0);         // one tile's addresses and addends at a time
             }
         }
