@@ -6,10 +6,10 @@
 // of the same rows, each with its own scale byte -- exactly the format's block, so no code is ever unpacked.  Products of codes are
 // exact; the sum is FP32.  D's layout: lane l holds column l & 31, rows 8 (e / 4) + 4 (l >> 5) + e % 4.
 //
-// MI355X: 8192^3 296 us = 3.7 PFLOP/s, 4.5 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
-// but these instructions makes 9.2, four times the BF16 rate of a large library product 4.8.  At 256 x 256 the instructions are 49 % of a
-// wave's cycles, 26 % are waits for panels out of L2 and at barriers.  One wave a tile with operands straight from memory, the first
-// form: 3.72 ms.
+// MI355X: 8192^3 282 us = 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
+// but these instructions makes 9.2, four times the BF16 rate of a large library product 4.8.  At 256 x 256 the instructions are half of a
+// wave's cycles, a quarter are waits for panels out of L2 and at barriers.  One wave a tile with operands straight from memory, the
+// first form: 3.72 ms.
 #include <cstdio>
 
 #include "activations.h"
@@ -501,6 +501,7 @@ static int launch_tile(const MxProductArgs &a, hipStream_t s)
 }
 
 // The tile, measured on MI355X (GPU time, both sides of each border):
+//   (both sides of a border from one build, whose epilogue took up to 15 % longer than this one's)
 //   rows    256 x 256 from k = 2048 on where it gives every CU a workgroup: 4096 x 16384 x 4096 185 us against 209 with 128 x 128 tiles, but
 //           4096 x 4096 x 1024 27.3 against 25.3 (one workgroup a CU hides neither end of a tile behind another)
 //           128 x 128 where it gives every CU two workgroups, or one from k = 2048 on: 512 x 8192 x 8192 31.1 us against 43.5 with 64 x 128
@@ -509,7 +510,7 @@ static int launch_tile(const MxProductArgs &a, hipStream_t s)
 //           else 64 x 64 (1024^3 5.6 us against 7.2 with 64 x 128)
 //   planes  64 x 128 where it gives every CU two workgroups, else 64 x 64: bound by the map's and the result's bytes and by the latency of
 //           gathering, they want waves (76 x 76 128 -> 256 3x3 of 64 images: 0.290 ms against 0.347 with 64 x 64; with 128 x 128 and 256 x 256
-//           1.1 and 1.9 times the time; 19 x 19 512 -> 1024 3x3 of 8 images 29.8 us with 64 x 64, 33.5 with 64 x 128)
+//           1.1 and 1.9 times the time; 19 x 19 512 -> 1024 3x3 of 8 images 30 us with 64 x 64, 33.5 with 64 x 128)
 template <int TYPE, bool CONV, bool BYTES>
 static int launch_by_size(const MxProductArgs &a, hipStream_t s, char *name, size_t name_len)
 {
