@@ -566,6 +566,21 @@ def test_rows_behind_the_last_are_not_read(mx, m, n, k, dtype):
     close(y, want, tol)
 
 
+@pytest.mark.parametrize("batch, c, n, h, w, size, stride, pad", [(1, 32, 33, 9, 9, 3, 1, 1), (2, 64, 70, 7, 5, 1, 1, 0), (1, 128, 100, 13, 13, 3, 2, 1), (3, 40, 255, 6, 6, 1, 1, 0), (8, 32, 41, 70, 70, 3, 1, 1)])
+def test_a_convolution_stays_inside_its_tensors(mx, batch, c, n, h, w, size, stride, pad):
+    x, f, *_ = conv_case(mx, batch, c, n, h, w, size, seed=c + n)
+    oh, ow = (h + 2 * pad - size) // stride + 1, (w + 2 * pad - size) // stride + 1
+    bias, res = rand(n, seed=1).cuda(), rand(batch, n, oh, ow, seed=2).cuda()
+    q, fq = mx.quantize_nchw(x), mx.quantize_filters(f)
+    want, side = mx.conv2d(q, fq, batch, h, w, size, stride, pad, bias=bias, activation="leaky", residual=res, want="both")
+    ends = [mx.Matrix(at_the_end(m.codes), at_the_end(m.scales), m.k) for m in (q, fq)]
+    got, side2 = mx.conv2d(*ends, batch, h, w, size, stride, pad, bias=at_the_end(bias), activation="leaky", residual=at_the_end(res), out=at_the_end(res), want="both")
+    kb = o.blocks(n)
+    assert torch.equal(got, want) and torch.equal(side.codes[:, :16 * kb], side2.codes[:, :16 * kb]) and torch.equal(side.scales[:, :kb], side2.scales[:, :kb])
+    plain = mx.conv2d(q, fq, batch, h, w, size, stride, pad)
+    assert torch.equal(mx.conv2d(*ends, batch, h, w, size, stride, pad, out=at_the_end(plain * 0)), plain)
+
+
 def test_gradients_are_refused(mx):
     from yolo2_light_amd import YoloHipError
     w, _ = make(mx, 8, 32, 1)

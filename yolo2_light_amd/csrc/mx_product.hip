@@ -140,7 +140,7 @@ __device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const m
     float y[16], add[16];
     mx_u32x4 b[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) b[q] = __builtin_amdgcn_raw_buffer_load_b128(bias, 16 * half, (ib + 8 * q) * 4, 0);      // zeros where there is none
+    for (int q = 0; q < 4; ++q) b[q] = __builtin_amdgcn_raw_buffer_load_b128(bias, (ib + 8 * q + 4 * half) * 4, 0, 0);   // zeros where there is none
     if (p.residual) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) add[e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(residual, off(e), row(e), 0));
