@@ -65,10 +65,12 @@ __device__ __forceinline__ void mx_unpack(mx_u32x4 x, float *v)
         }
     }
 }
+// vectors where memory has no more than the type's alignment: the hardware takes them
+typedef mx_u32x4 mx_u32x4_any __attribute__((aligned(2)));
 template <int TYPE>
-__device__ __forceinline__ mx_u32x4 mx_load_vec(const void *p, int64_t i) { return *reinterpret_cast<const mx_u32x4 *>(reinterpret_cast<const char *>(p) + i * (16 / MX_VEC<TYPE>)); }
+__device__ __forceinline__ mx_u32x4 mx_load_vec(const void *p, int64_t i) { return *reinterpret_cast<const mx_u32x4_any *>(reinterpret_cast<const char *>(p) + i * (16 / MX_VEC<TYPE>)); }
 template <int TYPE>
-__device__ __forceinline__ void mx_store_vec(void *p, int64_t i, mx_u32x4 v) { *reinterpret_cast<mx_u32x4 *>(reinterpret_cast<char *>(p) + i * (16 / MX_VEC<TYPE>)) = v; }
+__device__ __forceinline__ void mx_store_vec(void *p, int64_t i, mx_u32x4 v) { *reinterpret_cast<mx_u32x4_any *>(reinterpret_cast<char *>(p) + i * (16 / MX_VEC<TYPE>)) = v; }
 
 // activate(): LINEAR, LEAKY and RELU (x * (x > 0)) by one slope below zero, in 32 bits; the others only where RARE says so
 template <bool RARE>
@@ -112,9 +114,6 @@ __device__ __forceinline__ void mx_values8(unsigned codes, unsigned byte, float 
 __device__ __forceinline__ unsigned mx_abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
 __device__ __forceinline__ mx_v8i mx_operand(mx_v4i c) { return mx_v8i{c[0], c[1], c[2], c[3], 0, 0, 0, 0}; }
-
-// vectors where memory has no more than the type's alignment: the hardware takes them
-typedef mx_u32x4 mx_u32x4_any __attribute__((aligned(2)));
 
 // eight values from x[i], the first `n` of them; 16 bytes at a time where all eight are there
 template <int TYPE>

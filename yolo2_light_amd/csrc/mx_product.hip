@@ -6,7 +6,7 @@
 // of the same rows, each with its own scale byte -- exactly the format's block, so no code is ever unpacked.  Products of codes are
 // exact; the sum is FP32.  D's layout: lane l holds column l & 31, rows 8 (e / 4) + 4 (l >> 5) + e % 4.
 //
-// MI355X: 8192^3 282 us = 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
+// MI355X: 8192^3 280 to 292 us = 3.8 to 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
 // but these instructions makes 9.2, four times the BF16 rate of a large library product 4.8.  At 256 x 256 the instructions are half of a
 // wave's cycles, a quarter are waits for panels out of L2 and at barriers.  One wave a tile with operands straight from memory, the
 // first form: 3.72 ms.
@@ -37,9 +37,10 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_v4i a, mx_v4i b, mx_f32x16 c, in
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(a), mx_operand(b), c, 4, 4, S, sa, S, sb);
 }
 
-// A strip of D, 32 rows from ib by COLS columns from jb, in LDS: + bias, activation, + residual, to rows of memory.  In 16-byte vectors
-// where every row's begin on one, else by single values; AHEAD rows' addends are requested before the first is used.
-template <int TYPE, bool RARE, bool WIDE, int COLS, int PITCH>
+// A strip of D, 32 rows from ib by COLS columns from jb, in LDS: + bias, activation, + residual, to rows of memory.  WIDE: in 16-byte vectors,
+// wherever they begin (3420 x 15311 x 149 to BF16: 51 us by single values, which the rare activations are left with, 41 so), the
+// last of a row by its values; INSIDE: no column is behind a row's end; AHEAD rows' addends are requested before the first is used.
+template <int TYPE, bool RARE, bool WIDE, bool INSIDE, int COLS, int PITCH>
 __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const float *strip, int ib, int jb, int lane)
 {
     constexpr int VEC = WIDE ? MX_VEC<TYPE> : 1;
@@ -53,7 +54,8 @@ __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const flo
         if (j >= (int)p.J) return;
         float bias[VEC];
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) bias[q] = p.bias ? p.bias[j + q] : 0.f;
+        for (int q = 0; q < VEC; ++q) bias[q] = p.bias && (INSIDE || j + q < (int)p.J) ? p.bias[j + q] : 0.f;
+        const int n = INSIDE ? VEC : min(VEC, (int)p.J - j);
         const int r0 = lane / LANES;
         if (r0 >= rows) return;                            // and below: the first row of a step is always one of the matrix
         int64_t at = (int64_t)(ib + r0) * p.out_stride + j, res = (int64_t)(ib + r0) * p.residual_stride + j;
@@ -66,8 +68,9 @@ __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const flo
 #pragma unroll
                 for (int s = 0; s < AHEAD; ++s) {
                     const bool ok = r0 + (step + s) * ROWS < rows;
-                    if constexpr (WIDE) rv[s] = mx_load_vec<TYPE>(p.residual, ok ? res + s * res_step : res);
-                    else rs[s] = mx_load<TYPE>(p.residual, ok ? res + s * res_step : res);
+                    if constexpr (WIDE) {
+                        if (n == VEC) rv[s] = mx_load_vec<TYPE>(p.residual, ok ? res + s * res_step : res);
+                    } else rs[s] = mx_load<TYPE>(p.residual, ok ? res + s * res_step : res);
                 }
             }
 #pragma unroll
@@ -86,6 +89,14 @@ __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const flo
             for (int s = 0; s < AHEAD; ++s) {
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) v[s][q] = mx_activate<RARE>(v[s][q] + bias[q], act);
+                if (WIDE && n < VEC) {
+                    if (r0 + (step + s) * ROWS < rows) {
+#pragma unroll
+                        for (int q = 0; q < VEC; ++q)
+                            if (q < n) mx_store<TYPE>(p.out, at + s * out_step + q, add ? v[s][q] + mx_load<TYPE>(p.residual, res + s * res_step + q) : v[s][q]);
+                    }
+                    continue;
+                }
                 if (add) {
                     float r[8];
                     if constexpr (WIDE) mx_unpack<TYPE>(rv[s], r);
@@ -464,9 +475,6 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
         static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "strips fit in the panels' LDS");
         __syncthreads();
         float *strip = reinterpret_cast<float *>(smem) + wave * 32 * PITCH;
-        constexpr int VEC = MX_VEC<TYPE>;
-        const bool wide = p.J % VEC == 0 && p.out_stride % VEC == 0 && (uintptr_t)p.out % 16 == 0 &&
-                          (!p.residual || (p.residual_stride % VEC == 0 && (uintptr_t)p.residual % 16 == 0));
 #pragma unroll 1
         for (int t = 0; t < TI; ++t) {
 #pragma unroll
@@ -478,8 +486,8 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
                         for (int e = 0; e < 16; ++e) strip[(8 * (e / 4) + 4 * half + e % 4) * PITCH + tj * 32 + l31] = acc[ti][tj][e];
                 }
             const int ib = i0 + wi0 + t * 32;
-            if (ib < I && wide) mx_finish_rows<TYPE, RARE, !RARE, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
-            else if (ib < I) mx_finish_rows<TYPE, RARE, false, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
+            if (ib < I && j0 + wj0 + COLS <= J) mx_finish_rows<TYPE, RARE, !RARE, true, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
+            else if (ib < I) mx_finish_rows<TYPE, RARE, !RARE, false, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
         }
     }
 }
