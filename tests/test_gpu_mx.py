@@ -288,7 +288,8 @@ def test_extreme_scales(mx):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("m, n, k", [s for s in SIZES if s[0] * s[1] * s[2] < 40_000_000] + [(1, 4096, 4096), (4, 2050, 4100), (48, 512, 2048), (600, 130, 200)])
+@pytest.mark.parametrize("m, n, k", [s for s in SIZES if s[0] * s[1] * s[2] < 40_000_000] + [(1, 4096, 4096), (4, 2050, 4100), (48, 512, 2048), (600, 130, 200),
+                         (1, 33, 76_800), (1, 33, 76_801), (2, 40, 16_384), (2, 40, 16_385), (16, 40, 2048), (16, 40, 2049), (17, 8200, 96), (5, 8200, 100)])      # borders of the forms
 def test_linear_is_matmul_of_the_rounded_rows(mx, m, n, k, dtype):
     x = rand(m, k + 3, seed=m + k, dtype=dtype).cuda()[:, 1:k + 1]
     w, _ = make(mx, n, k, n)
