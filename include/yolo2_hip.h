@@ -521,7 +521,8 @@ int yl_mx_matmul(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
 
 /* yl_mx_matmul on yl_mx_quantize(x), the same bits, in one call.  x: batch 1.  `workspace` is device memory of at least
  * yl_mx_linear_workspace(x->rows, x->k) bytes, 16-byte aligned, which holds the rounded x while the call runs: calls that may run
- * at the same time need one each.  (It is 0 where the product rounds x itself: a few rows, the single token of a decoding step.) */
+ * at the same time need one each.  (It is 0 where the product rounds x itself -- a few rows, the single token of a decoding step -- and
+ * for an x of more than 2^46 blocks, which yl_mx_linear refuses.) */
 int64_t yl_mx_linear_workspace(int64_t rows, int64_t k);
 int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix *w, const yl_mx_epilogue *epilogue, const yl_dense *y,
                  void *workspace, int64_t workspace_bytes);

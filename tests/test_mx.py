@@ -178,6 +178,15 @@ def test_refused_linear_layers():
         accepted(linear(x=dense(**big), y=wide))
 
 
+def test_refused_inputs_that_no_workspace_holds():
+    """A broadcast row has any number of rows; the workspace of 0 bytes of such an x is not the one of an x that is rounded in the product."""
+    for rows, k in ((1 << 29, 1 << 23), (2 ** 31 - 300, 1 << 21), (1 << 31 >> 1, 1 << 22)):
+        assert lib.yl_mx_linear_workspace(rows, k) == 0
+        w, y = dict(rows=1, k=k, ld=k // 32, codes=1 << 40, scales=1 << 41), dict(rows=rows, k=1, data=1 << 42)
+        for ws, ws_bytes in ((None, 0), (1 << 44, 1 << 43)):
+            refused(linear(x=dense(rows=rows, k=k, rs=0), w=w, y=y, ws=ws, ws_bytes=ws_bytes), "too large")
+
+
 def conv(x=None, f=None, shape=(1, 4, 4, 3, 1, 1), e=None, out=96 * MB, q=None, device=0):
     x = matrix(rows=16, k=32, ld=1) if x is None else x
     f = matrix(rows=8, k=9 * 32, ld=12, codes=64 * MB, scales=80 * MB) if f is None else f

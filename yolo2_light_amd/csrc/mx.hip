@@ -234,7 +234,9 @@ int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix
     const int64_t xe = type_bytes(x->type), ye = type_bytes(y->type);
     const bool apart = x->k_stride == 1 && x->row_stride * xe == y->row_stride * ye && beside(x->data, x->k * xe, y->data, y->k * ye, y->row_stride * ye);
     if (!apart && out.meets(in)) return refuse(entry, "y overlaps x");
+    const bool fused = mx_linear_fused(x->rows, x->k), some = x->rows > 0 && x->k > 0;
     const int64_t need = yl_mx_linear_workspace(x->rows, x->k);
+    if (some && !fused && need == 0) return refuse(entry, "x is too large for a workspace");
     if (need > 0) {
         if (!workspace || workspace_bytes < need) return refuse(entry, "workspace is smaller than yl_mx_linear_workspace(x->rows, x->k)");
         if ((uintptr_t)workspace % 16) return refuse(entry, "workspace is not 16-byte aligned");
@@ -248,7 +250,7 @@ int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix
     DeviceScope scope;
     if (int rc = scope.enter(entry, device)) return rc;
     if (x->rows == 0 || w->rows == 0) return YL_OK;
-    if (x->k > 0 && need == 0) return launched(entry, launch_mx_linear(a, dense_of(x), stream));
+    if (some && fused) return launched(entry, launch_mx_linear(a, dense_of(x), stream));
     const int64_t ld = yl_mx_blocks(x->k);
     a.a_codes = workspace; a.a_scales = (char *)workspace + x->rows * ld * 16; a.a_ld = ld;
     if (int rc = launched(entry, launch_mx_quantize(dense_of(x), workspace, (char *)workspace + x->rows * ld * 16, ld, stream))) return rc;
