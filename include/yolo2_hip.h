@@ -347,7 +347,8 @@ int yl_network_set_variant(yl_network *net, int bits);
  * "strict_fp32"). */
 #define YL_PRECISION_FP32_STRICT 2
 /* Opt-in MXFP4 variant of the FP32 path (BEFORE yl_network_to_device): the convolutions that `quantized` would run in INT8 under
- * YL_QUANT_RULE_CPU (not the first layer, not linear heads) and whose input has whole blocks of 32 channels run as yl_mx_conv2d:
+ * YL_QUANT_RULE_CPU (not the first layer, not linear heads), whose input has whole blocks of 32 channels and whose sizes yl_mx_conv2d
+ * takes (the others stay FP32; yl_network_layer_info's info[16] says which) run as yl_mx_conv2d:
  * input and weights rounded to MXFP4 (yl_mx_quantize's rule, no calibration), FP32 accumulation, bias, activation and fused
  * [shortcut]; with yl_network_set_fusion the rounded input of a layer is written by the convolution in front of it.  Rounding to
  * 4 bits is far outside the FP32 path's contract: a network has to be trained or tuned for it. */

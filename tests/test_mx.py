@@ -219,6 +219,38 @@ def test_refused_convolutions():
         accepted(conv(x=matrix(rows=0, k=32, ld=1), shape=(0, 4, 4, 3, 1, 1)))
 
 
+def conv_taken(batch, h, w, c, n, size, stride, pad):
+    """yl_mx_conv2d takes these sizes (all pointers far from one another); None: refused."""
+    rows, taps, oh, ow = batch * h * w, size * size, (h + 2 * pad - size) // stride + 1, (w + 2 * pad - size) // stride + 1
+    x = matrix(rows=rows, k=c, ld=c // 32, codes=1 << 50, scales=1 << 52)
+    f = matrix(rows=n, k=taps * c, ld=lib.yl_mx_blocks(taps * c), codes=1 << 54, scales=1 << 55)
+    assert n * batch * oh * ow < 1 << 46
+    rc = conv(x=x, f=f, shape=(batch, h, w, size, stride, pad), out=1 << 57, q=matrix(rows=batch * oh * ow, k=n, ld=(n + 31) // 32, codes=1 << 59, scales=1 << 61))
+    assert rc in (ARG, DEVICE)
+    return rc == DEVICE
+
+
+@pytest.mark.skipif(HAVE_GPU, reason="asks the entry for sizes without memory behind them: ends at the missing device")
+@pytest.mark.parametrize("batch, h, w, c, n, size, stride, pad, takes", [
+    (1, 608, 608, 32, 64, 3, 2, 1, True), (64, 608, 608, 32, 64, 3, 2, 1, True), (1, 8224, 8224, 32, 64, 3, 2, 1, False),     # planes above 2^32 bytes
+    (1, 4096, 4096, 32, 31, 1, 1, 0, True), (1, 4096, 4096, 32, 32, 1, 1, 0, False), (1, 4096, 4096, 32, 33, 1, 1, 0, False),  # around 2 GB
+    (1, 20000, 20000, 32, 1, 3, 1, 1, False), (3, 20000, 20000, 32, 1, 3, 1, 1, False),                                        # an image's pixels above 2^28
+    (8, 16000, 16000, 32, 1, 3, 1, 1, True), (9, 16000, 16000, 32, 1, 3, 1, 1, False),                                         # positions around 2^31
+    (1, 1 << 20, 32, 32, 2, 3, 1, 1, True), (1, (1 << 20) + 1, 32, 32, 2, 3, 1, 1, False), (2, 13, 1 << 20, 64, 1, 3, 2, 1, True),
+    (1, 60, 1 << 20, 512, 1, 3, 1, 1, False), (4, 13, 13, 1 << 14, 64, 3, 1, 1, True), (4, 5, 5, (1 << 18) + 32, 8, 1, 1, 0, False)])
+def test_a_network_takes_the_sizes_that_the_operator_takes(batch, h, w, c, n, size, stride, pad, takes):
+    """A layer beyond the kernel's 32-bit offsets stays in FP32; in MXFP4 its last filters once wrapped onto the first, without an error."""
+    from yolo2_light_amd import Network
+    import descs as D
+    assert conv_taken(batch, h, w, c, n, size, stride, pad) == takes
+    zeros = np.zeros(max(c, n * c * size * size), np.float32)
+    first = D.conv(batch, w, h, 1, c, 1, 1, 0, D.LEAKY, zeros[:c], zeros[:c])
+    net = Network.from_desc([first, D.conv(batch, w, h, c, n, size, stride, pad, D.LEAKY, zeros[:n * c * size * size], zeros[:n])], batch, w, h, 1)
+    net.set_precision(3)
+    assert [li["conv_mode"] for li in net.layers()] == [0, 4 if takes else 0]
+    net.close()
+
+
 def test_as_many_rows_as_32_bits_count():
     most = 0x7fffffff - 256
     for x, y in ((dict(rows=most + 1, k=32, ld=1), dict(rows=most + 1, k=1, data=1 << 50)), (dict(rows=1, k=32, ld=1), dict(rows=1, k=most + 1, data=1 << 50))):

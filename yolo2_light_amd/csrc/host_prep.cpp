@@ -10,6 +10,7 @@
 //   get_distribution / get_multiplier / max_abs             src/yolov2_forward_network_quantized.c:35-87 / 23-27
 // The device-side layouts (k-major FP32 panels, channel-fastest INT8, 64-bit
 // sign words) are built from these host arrays in runtime.hip.
+#include "mx.h"
 #include "yl_internal.h"
 
 #include <cmath>
@@ -167,9 +168,11 @@ void select_conv_modes(Network &net) {
         // opt-in (yl_network_set_precision): FP32 convolutions with whole 8-channel groups take bf16 operands
         else if (net.precision == YL_PRECISION_BF16 && !l.xnor && (l.c % 8) == 0 && l.size <= 5) l.conv_mode = CONV_BF16;
         // opt-in: MXFP4 operands for the convolutions that the CPU rule above would run in INT8 (not the first, not linear heads), where
-        // whole blocks of 32 channels come in
-        else if (net.precision == YL_PRECISION_MXFP4 && !l.xnor && i >= 1 && l.activation != YL_LINEAR && (l.c % 32) == 0 && l.size <= 5 &&
-                 l.pad >= 0 && l.pad < l.size) l.conv_mode = CONV_MX4;
+        // whole blocks of 32 channels come in and the kernel's 32-bit offsets hold the sizes (FP32 beyond them: an image's result of 2 GB, say)
+        else if (net.precision == YL_PRECISION_MXFP4 && !l.xnor && i >= 1 && l.activation != YL_LINEAR && l.c > 0 && (l.c % MX_BLOCK) == 0 &&
+                 l.size >= 1 && l.size <= MX_MAX_SIZE && l.pad >= 0 && l.pad < l.size && l.stride >= 1 && l.h >= 1 && l.w >= 1 &&
+                 l.h + 2 * l.pad >= l.size && l.w + 2 * l.pad >= l.size &&
+                 !mx_conv_beyond(net.batch, l.h, l.w, l.c, l.c / MX_BLOCK, l.n, l.size, l.stride, l.pad)) l.conv_mode = CONV_MX4;
         else l.conv_mode = CONV_F32;
     }
 }

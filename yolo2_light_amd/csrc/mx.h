@@ -8,6 +8,27 @@ namespace yl {
 constexpr int MX_BLOCK = 32;       // values a scale covers; 16 bytes of codes
 constexpr int MX_MAX_SIZE = 5;     // filter edge: the taps' validity is a 25-bit mask
 
+constexpr int64_t MX_MAX_ELEMENTS = (int64_t)1 << 46;     // what a stride or a size may address: products of two stay in 64 bits
+constexpr int64_t MX_MAX_ROWS = 0x7fffffff - 256;         // rows of a product's side: the end of a tile of 256 is still a 32-bit number
+
+// Why the kernel's 32-bit counts and offsets do not hold a convolution (of a map of `c` channels, x_ld blocks from pixel to pixel, with n
+// filters), or nullptr.  0 <= pad < size, 1 <= h, w, c, stride, and the filter is no larger than the padded map.
+inline const char *mx_conv_beyond(int64_t batch, int64_t h, int64_t w, int64_t c, int64_t x_ld, int64_t n, int size, int64_t stride, int pad)
+{
+    if (h > 1 << 20 || w > 1 << 20 || stride > 1 << 20) return "a map edge or stride above 2^20";
+    if (c > 1 << 18) return "more than 2^18 channels";
+    if (n > MX_MAX_ROWS || batch > MX_MAX_ROWS / (h * w)) return "map or result is too large";
+    const int64_t oh = (h + 2 * pad - size) / stride + 1, ow = (w + 2 * pad - size) / stride + 1, area = oh * ow;
+    if (batch > MX_MAX_ROWS / area || (batch > 0 && n > MX_MAX_ELEMENTS / (batch * area))) return "map or result is too large";
+    // the rows of the map under 256 neighbouring positions of the result
+    const int64_t rows = batch * h * w, under = (size + 1) * (w + 1), part = 256 % area;
+    const int64_t reach = (256 / area + 1) * h * w + ((part + ow - 1) / ow + 1) * stride * w + under;
+    if ((reach < rows ? reach : rows) + under > 0xFFFFFFFFLL / 16 / x_ld) return "rows of the map are too far apart";
+    // the planes of the images that 256 neighbouring positions lie in
+    if ((256 / area + 2) > 0xFFFFFFFFLL / 4 / (area * (n > 0 ? n : 1))) return "an image's result is too large";
+    return nullptr;
+}
+
 struct MxDense {                   // see yl_dense
     const void *data;
     int type;

@@ -9,10 +9,7 @@
 namespace yl {
 namespace {
 
-constexpr int64_t MX_MAX_ELEMENTS = (int64_t)1 << 46;     // what a stride or a size may address: products of two stay in 64 bits
 constexpr int64_t MX_MAX_LD = (int64_t)1 << 19;           // blocks a row: 32-bit offsets inside a tile of 256 rows
-
-constexpr int64_t MX_MAX_ROWS = 0x7fffffff - 256;         // rows of a product's side: the end of a tile of 256 is still a 32-bit number
 
 // nothing may be thrown through a C entry: an error text that finds no memory is left out
 int refuse(const char *entry, const char *what, int rc = YL_ERR_ARG) noexcept
@@ -269,19 +266,15 @@ int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
     if (c.batch < 0 || c.h < 1 || c.w < 1 || c.size < 1 || c.size > MX_MAX_SIZE || c.stride < 1 || c.pad < 0 || c.pad >= c.size)
         return refuse(entry, "shape: batch >= 0, h, w >= 1, 1 <= size <= 5, stride >= 1, 0 <= pad < size");
     if (x->k < 1 || c.h > 1 << 20 || c.w > 1 << 20 || c.stride > 1 << 20) return refuse(entry, "no channels, or a map edge or stride above 2^20");
-    if (x->rows != (int64_t)c.batch * c.h * c.w) return refuse(entry, "x is not batch * h * w rows");
+    const int64_t pixels = (int64_t)c.h * c.w;
+    if (c.batch > MX_MAX_ELEMENTS / pixels) return refuse(entry, "map or result is too large");
+    if (x->rows != c.batch * pixels) return refuse(entry, "x is not batch * h * w rows");
     if (filters->k != (int64_t)c.size * c.size * blocks_of(x->k) * MX_BLOCK) return refuse(entry, "filters' k is not size * size * whole blocks of x's channels");
     const int oh_num = c.h + 2 * c.pad - c.size, ow_num = c.w + 2 * c.pad - c.size;
     if (oh_num < 0 || ow_num < 0) return refuse(entry, "the filter is larger than the padded map");
+    if (const char *m = mx_conv_beyond(c.batch, c.h, c.w, x->k, x->ld, filters->rows, c.size, c.stride, c.pad)) return refuse(entry, m);
     const int oh = oh_num / c.stride + 1, ow = ow_num / c.stride + 1;
     const int64_t J = (int64_t)c.batch * oh * ow, I = filters->rows;
-    if (J > MX_MAX_ROWS || I > MX_MAX_ROWS || x->rows > MX_MAX_ROWS || (J > 0 && I > MX_MAX_ELEMENTS / J)) return refuse(entry, "map or result is too large");
-    // the kernels' 32-bit offsets: the rows of the map under 256 neighbouring positions of the result
-    const int64_t area = (int64_t)oh * ow, part = 256 % area;
-    const int64_t reach = (256 / area + 1) * c.h * c.w + ((part + ow - 1) / ow + 1) * c.stride * c.w + (int64_t)(c.size + 1) * (c.w + 1);
-    if ((reach < x->rows ? reach : x->rows) + (int64_t)(c.size + 1) * (c.w + 1) > 0xFFFFFFFFLL / 16 / x->ld) return refuse(entry, "rows of the map are too far apart");
-    if (x->k > 1 << 18) return refuse(entry, "more than 2^18 channels");
-    if ((256 / area + 2) > 0xFFFFFFFFLL / 4 / (area * (I > 0 ? I : 1))) return refuse(entry, "an image's result is too large");
     const float *bias = epilogue ? epilogue->bias : nullptr;
     const float *residual = epilogue ? (const float *)epilogue->residual : nullptr;
     if ((uintptr_t)out % 4 || (uintptr_t)residual % 4) return refuse(entry, "out or residual is not aligned to its type");
