@@ -276,6 +276,20 @@ def test_empty_products(mx):
     assert (y == b.expand(300, 40)).all()
 
 
+@pytest.mark.parametrize("lead", [(2, 3), (1, 2, 2), (7,), ()])
+def test_nothing_to_sum_under_any_leading_axes(mx, lead):
+    """x [..., 0]: every row of the result is activation(bias) + residual."""
+    m, n = int(np.prod(lead)), 40
+    b, res = rand(n, seed=1).cuda(), rand(m, n, seed=2).reshape(*lead, n).cuda()
+    w = mx.Matrix.empty(n, 0, "cuda")
+    out = torch.full((*lead, n), float("nan"), device="cuda")
+    y = mx.linear(torch.empty(*lead, 0, device="cuda"), w, bias=b, activation="relu", residual=res, out=out)
+    assert torch.equal(y, b.clamp(min=0) + res)
+    q = mx.quantize(torch.empty(*lead, 0, device="cuda"))
+    assert (q.rows, q.k) == (m, 0) and mx.dequantize(q).shape == (m, 0)
+    assert mx.linear(torch.ones(*lead, 64, device="cuda"), mx.Matrix.empty(0, 64, "cuda")).shape == (*lead, 0)
+
+
 def test_extreme_scales(mx):
     """2^100 against 2^-100, and sums that leave FP32."""
     x, xv = make(mx, 70, 256, 1, spread=0.2)

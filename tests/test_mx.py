@@ -272,3 +272,11 @@ def test_python_refuses_what_is_not_on_a_gpu():
                  lambda: mx.Matrix(x, x, 64), lambda: mx.matmul(x, x), lambda: mx.conv2d(x, x, 1, 2, 2, 1), lambda: mx.dequantize(x)):
         with pytest.raises(YoloHipError):
             call()
+
+
+def test_python_counts_the_rows_of_empty_tensors():
+    torch = pytest.importorskip("torch")
+    from yolo2_light_amd import mx
+    for shape in ((2, 3, 0), (2, 0, 3), (0, 3, 5), (3, 0), (0, 3), (2, 3, 4, 0), (2, 3, 4)):
+        d = mx._rows_of(torch.zeros(shape), "x")
+        assert (d.rows, d.k) == (int(np.prod(shape[:-1])), shape[-1]), shape

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 from typing import Optional
 
 import torch
@@ -130,7 +131,7 @@ def _rows_of(x, name: str) -> Dense:
     if len(shape) == 1:
         return Dense(x.data_ptr(), kind, 1, 1, shape[0], 0, 0, x.stride(0))
     try:
-        flat = x.view(-1, shape[-1]) if x.numel() else x.reshape(0, shape[-1])
+        flat = x.view(-1, shape[-1]) if x.numel() else x.reshape(math.prod(shape[:-1]), shape[-1])
     except RuntimeError:
         _fail("the leading axes of %s cannot be taken as one axis of rows: make it contiguous" % name)
     return Dense(x.data_ptr(), kind, 1, flat.shape[0], shape[-1], 0, flat.stride(0), x.stride(-1))
