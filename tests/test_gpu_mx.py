@@ -290,6 +290,12 @@ def test_nothing_to_sum_under_any_leading_axes(mx, lead):
     assert mx.linear(torch.ones(*lead, 64, device="cuda"), mx.Matrix.empty(0, 64, "cuda")).shape == (*lead, 0)
 
 
+def test_no_filters_or_no_channels(mx):
+    for shape in ((0, 64, 3, 3), (5, 0, 3, 3), (0, 0, 1, 1)):
+        f = mx.quantize_filters(torch.zeros(shape, device="cuda"))
+        assert (f.rows, f.k) == (shape[0], shape[2] * shape[3] * ((shape[1] + 31) // 32 * 32))
+
+
 def test_extreme_scales(mx):
     """2^100 against 2^-100, and sums that leave FP32."""
     x, xv = make(mx, 70, 256, 1, spread=0.2)

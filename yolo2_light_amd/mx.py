@@ -177,7 +177,7 @@ def quantize_filters(w) -> Matrix:
     n, c, size, _ = w.shape
     rows = torch.zeros(n, size, size, (c + BLOCK - 1) // BLOCK * BLOCK, dtype=w.dtype, device=w.device)
     rows[..., :c] = w.permute(0, 2, 3, 1)
-    return quantize(rows.view(n, -1))
+    return quantize(rows.view(n, rows.shape[1] * rows.shape[2] * rows.shape[3]))
 
 
 def _dequantize(q: Matrix, out, dst: Dense):
