@@ -475,6 +475,13 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
         static_assert(4 * 32 * PITCH * 4 <= 2 * STAGE, "strips fit in the panels' LDS");
         __syncthreads();
         float *strip = reinterpret_cast<float *>(smem) + wave * 32 * PITCH;
+        // A strip passes between the lanes of its wave alone.  The wave's LDS operations end in the order they were issued in; that the
+        // compiler issues a lane's reads behind the other lanes' stores, and the next strip's stores behind the reads, is said here.
+        auto wave_order = [] {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
 #pragma unroll 1
         for (int t = 0; t < TI; ++t) {
 #pragma unroll
@@ -485,9 +492,11 @@ __global__ __launch_bounds__(MX_THREADS, TI + TJ > 4 ? 1 : CONV && TI == TJ && !
 #pragma unroll
                         for (int e = 0; e < 16; ++e) strip[(8 * (e / 4) + 4 * half + e % 4) * PITCH + tj * 32 + l31] = acc[ti][tj][e];
                 }
+            wave_order();
             const int ib = i0 + wi0 + t * 32;
             if (ib < I && j0 + wj0 + COLS <= J) mx_finish_rows<TYPE, RARE, !RARE, true, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
             else if (ib < I) mx_finish_rows<TYPE, RARE, !RARE, false, COLS, PITCH>(p, strip, ib, j0 + wj0, lane);
+            wave_order();
         }
     }
 }
