@@ -612,6 +612,23 @@ def test_gradients_are_refused(mx):
         assert mx.linear(x, w).shape == (2, 8)
 
 
+def test_negated_views_are_refused(mx):
+    """z.conj().imag shares z's memory, which holds the negatives of its values."""
+    from yolo2_light_amd import YoloHipError
+    w, _ = make(mx, 8, 64, 1)
+    z = torch.complex(rand(8, 64, seed=1), rand(8, 64, seed=2)).cuda().conj()
+    x, one = z.imag, torch.complex(torch.zeros(1), torch.ones(1)).cuda().conj().imag
+    assert x.is_neg() and one.is_neg() and one.is_contiguous()
+    plain = x.resolve_neg()
+    check_matrix(mx.quantize(plain), f64(plain))
+    m = z.view(1, 8, 8, 8).imag
+    for call in (lambda: mx.quantize(x), lambda: mx.linear(x, w), lambda: mx.quantize_nchw(m), lambda: mx.quantize_filters(m), lambda: mx.dequantize(w, out=x),
+                 lambda: mx.linear(plain, w, residual=x[:, :8]), lambda: mx.linear(plain, w, out=x[:, :8]), lambda: mx.linear(plain, w, bias=one.expand(8)),
+                 lambda: mx.linear(plain[:, :64], mx.Matrix(w.codes[:1], w.scales[:1], 64), bias=one)):
+        with pytest.raises(YoloHipError, match="resolve_neg"):
+            call()
+
+
 def test_python_refusals(mx):
     from yolo2_light_amd import YoloHipError
     w, _ = make(mx, 8, 64, 1)

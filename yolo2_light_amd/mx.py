@@ -31,7 +31,8 @@ def _fail(what: str):
 
 
 def _tensor(t, name: str, device: Optional[int] = None) -> int:
-    """The index of the GPU that t is on; -> raises unless t is a tensor on a GPU (on `device`, if given) that needs no gradient."""
+    """The index of the GPU that t is on; -> raises unless t is a tensor on a GPU (on `device`, if given) that needs no gradient and
+    whose memory holds its values."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _fail("%s is not a tensor on a GPU" % name)
     at = t.get_device()
@@ -39,6 +40,8 @@ def _tensor(t, name: str, device: Optional[int] = None) -> int:
         _fail("%s is on cuda:%d, not on cuda:%d" % (name, at, device))
     if t.requires_grad and torch.is_grad_enabled():
         _fail("%s requires a gradient, and there is no backward pass: detach it, or call under torch.no_grad()" % name)
+    if t.is_neg():
+        _fail("%s is a view that stands for the negatives of what its memory holds: call resolve_neg()" % name)
     return at
 
 
