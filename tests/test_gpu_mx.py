@@ -612,6 +612,25 @@ def test_gradients_are_refused(mx):
         assert mx.linear(x, w).shape == (2, 8)
 
 
+def test_tangents_are_refused(mx):
+    """A dual tensor of forward mode does not require a gradient; its result would have lost the tangent."""
+    from torch.autograd import forward_ad
+    from yolo2_light_amd import YoloHipError
+    w, _ = make(mx, 8, 64, 1)
+    x, b = torch.ones(2, 64, device="cuda"), torch.ones(8, device="cuda")
+    want = mx.linear(x, w, bias=b)
+    with forward_ad.dual_level():
+        d, db, m = forward_ad.make_dual(x, x), forward_ad.make_dual(b, b), forward_ad.make_dual(x.view(1, 32, 2, 2), x.view(1, 32, 2, 2))
+        for call in (lambda: mx.quantize(d), lambda: mx.linear(d[:1], w), lambda: mx.linear(x, w, bias=db), lambda: mx.quantize_nchw(m), lambda: mx.quantize_filters(m),
+                     lambda: mx.linear(x, w, residual=db.expand(2, 8)), lambda: mx.linear(x, w, out=db.expand(2, 8).contiguous())):
+            with pytest.raises(YoloHipError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(YoloHipError, match="tangent"):
+                call()
+        assert torch.equal(mx.linear(x, w, bias=b), want) and torch.equal(mx.linear(forward_ad.unpack_dual(d).primal, w, bias=b), want)
+    assert torch.equal(mx.linear(x, w, bias=b), want)
+
+
 def test_negated_views_are_refused(mx):
     """z.conj().imag shares z's memory, which holds the negatives of its values."""
     from yolo2_light_amd import YoloHipError

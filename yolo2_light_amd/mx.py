@@ -6,8 +6,8 @@
     f = mx.quantize_filters(weights)           # [n, c, size, size] -> Matrix
     y = mx.conv2d(mx.quantize_nchw(x), f, batch, h, w, size, stride, pad, bias=b, activation="leaky", residual=r)
 
-Every call runs on the current stream of its tensors' device and returns without waiting.  There is no backward pass: a call on a
-tensor that requires a gradient raises.  Plumbing only: all arithmetic happens in libyolo2hip.so."""
+Every call runs on the current stream of its tensors' device and returns without waiting.  There are no derivatives: a call on a
+tensor that requires a gradient, or that carries a tangent of forward mode, raises.  Plumbing only: all arithmetic happens in libyolo2hip.so."""
 from __future__ import annotations
 
 import ctypes as C
@@ -16,6 +16,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import Dense, MxConv, MxEpilogue, MxMatrix, YoloHipError, lib, check
 
@@ -40,6 +41,8 @@ def _tensor(t, name: str, device: Optional[int] = None) -> int:
         _fail("%s is on cuda:%d, not on cuda:%d" % (name, at, device))
     if t.requires_grad and torch.is_grad_enabled():
         _fail("%s requires a gradient, and there is no backward pass: detach it, or call under torch.no_grad()" % name)
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _fail("%s carries a tangent, and there is no forward-mode derivative: unpack it" % name)
     if t.is_neg():
         _fail("%s is a view that stands for the negatives of what its memory holds: call resolve_neg()" % name)
     return at
