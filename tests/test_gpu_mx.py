@@ -631,6 +631,27 @@ def test_tangents_are_refused(mx):
     assert torch.equal(mx.linear(x, w, bias=b), want)
 
 
+def test_autograd_knows_of_results_written_into_given_tensors(mx):
+    """y = a * buffer keeps the buffer for its backward pass; a call that writes the buffer in between must not go unseen."""
+    w, _ = make(mx, 8, 64, 1)
+    x, img = rand(2, 64, seed=2).cuda(), rand(1, 64, 3, 3, seed=3).cuda()
+    q, qi, f = mx.quantize(x), mx.quantize_nchw(img), mx.quantize_filters(rand(8, 64, 1, 1, seed=4).cuda())
+    for shape, write in (((2, 8), lambda out: mx.linear(x, w, out=out)), ((2, 8), lambda out: mx.matmul(q, w, out=out)), ((2, 64), lambda out: mx.dequantize(q, out=out)),
+                         ((1, 64, 3, 3), lambda out: mx.dequantize_nchw(qi, 1, 3, 3, out=out)), ((1, 8, 3, 3), lambda out: mx.conv2d(qi, f, 1, 3, 3, 1, out=out))):
+        a, buffer = torch.ones(shape, device="cuda", requires_grad=True), torch.ones(shape, device="cuda")
+        y = (a * buffer).sum()
+        write(buffer)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        (a * buffer).sum().backward()                             # with what is there now
+        assert torch.equal(a.grad, buffer)
+        with torch.inference_mode():
+            write(torch.empty(shape, device="cuda"))
+    before = q.codes._version, q.scales._version
+    mx.quantize(x, out=q)
+    assert q.codes._version > before[0] and q.scales._version > before[1]
+
+
 def test_negated_views_are_refused(mx):
     """z.conj().imag shares z's memory, which holds the negatives of its values."""
     from yolo2_light_amd import YoloHipError

@@ -118,6 +118,13 @@ class Matrix:
         return self._codes.device
 
 
+def _written(*tensors):
+    """Results went into tensors of the caller's: autograd has to know, or a backward pass that saved one computes with what is there now."""
+    for t in tensors:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
 def _matrix(m, name: str, device: Optional[int] = None) -> int:
     if not isinstance(m, Matrix):
         _fail("%s is not an mx.Matrix" % name)
@@ -155,12 +162,15 @@ def _map_of(x, name: str) -> Dense:
 
 
 def _quantize(src: Dense, device: int, out: Optional[Matrix]) -> Matrix:
-    if out is None:
-        out = Matrix.empty(src.batch * src.rows, src.k, _gpu(device))
+    q = out
+    if q is None:
+        q = Matrix.empty(src.batch * src.rows, src.k, _gpu(device))
     else:
-        _matrix(out, "out", device)
-    check(lib.yl_mx_quantize(device, _stream(device), _ref(src), _ref(out._c)), "yl_mx_quantize")
-    return out
+        _matrix(q, "out", device)
+    check(lib.yl_mx_quantize(device, _stream(device), _ref(src), _ref(q._c)), "yl_mx_quantize")
+    if out is not None:
+        _written(out._codes, out._scales)
+    return q
 
 
 def quantize(x, out: Optional[Matrix] = None) -> Matrix:
@@ -186,29 +196,33 @@ def quantize_filters(w) -> Matrix:
     return quantize(rows.view(n, rows.shape[1] * rows.shape[2] * rows.shape[3]))
 
 
-def _dequantize(q: Matrix, out, dst: Dense):
+def _dequantize(q: Matrix, out, dst: Dense, given: bool):
     check(lib.yl_mx_dequantize(q.index, _stream(q.index), _ref(q._c), _ref(dst)), "yl_mx_dequantize")
+    if given:
+        _written(out)
     return out
 
 
 def dequantize(q: Matrix, dtype=torch.float32, out=None):
     """The values of q, [rows, k]."""
     device = _matrix(q, "q")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((q.rows, q.k), dtype=dtype, device=_gpu(device))
     else:
         _tensor(out, "out", device)
-    return _dequantize(q, out, _rows_of(out, "out"))
+    return _dequantize(q, out, _rows_of(out, "out"), given)
 
 
 def dequantize_nchw(q: Matrix, batch: int, h: int, w: int, dtype=torch.float32, out=None):
     """The values of a quantised map, [batch, q.k, h, w]."""
     device = _matrix(q, "q")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((batch, q.k, h, w), dtype=dtype, device=_gpu(device))
     else:
         _tensor(out, "out", device)
-    return _dequantize(q, out, _map_of(out, "out"))
+    return _dequantize(q, out, _map_of(out, "out"), given)
 
 
 def _epilogue(n: int, device: int, bias, activation, residual) -> Optional[MxEpilogue]:
@@ -259,8 +273,10 @@ def matmul(x: Matrix, w: Matrix, bias=None, activation="linear", residual=None, 
     """activation(x w^T + bias) + residual, [x.rows, w.rows]."""
     device = _matrix(x, "x")
     _matrix(w, "w", device)
+    given = out
     out, y, e = _linear_args((x.rows,), x.rows, w, device, bias, activation, residual, dtype, out)
     check(lib.yl_mx_matmul(device, _stream(device), _ref(x._c), _ref(w._c), None if e is None else _ref(e), _ref(y)), "yl_mx_matmul")
+    _written(given)
     return out
 
 
@@ -270,12 +286,13 @@ def linear(x, w: Matrix, bias=None, activation="linear", residual=None, dtype=No
     device = _tensor(x, "x")
     _matrix(w, "w", device)
     xd = _rows_of(x, "x")
-    m = xd.rows
+    m, given = xd.rows, out
     out, y, e = _linear_args(x.shape[:-1], m, w, device, bias, activation, residual, dtype or x.dtype, out)
     need = lib.yl_mx_linear_workspace(m, xd.k)
     ws = torch.empty(need, dtype=torch.uint8, device=_gpu(device)) if need else None
     check(lib.yl_mx_linear(device, _stream(device), _ref(xd), _ref(w._c), None if e is None else _ref(e), _ref(y),
                            ws.data_ptr() if need else None, need), "yl_mx_linear")
+    _written(given)
     return out
 
 
@@ -294,6 +311,7 @@ def conv2d(x: Matrix, filters: Matrix, batch: int, h: int, w: int, size: int, st
         _tensor(residual, "residual", device)
         if residual.dtype is not torch.float32 or residual.shape != (batch, n, oh, ow) or not residual.is_contiguous():
             _fail("residual is a contiguous float32 tensor of the result's shape")
+    given = out
     if want == "mx":
         if out is not None:
             _fail("out is given, but want is \"mx\"")
@@ -308,4 +326,5 @@ def conv2d(x: Matrix, filters: Matrix, batch: int, h: int, w: int, size: int, st
     shape = MxConv(batch, h, w, size, stride, pad)
     check(lib.yl_mx_conv2d(device, _stream(device), _ref(x._c), _ref(filters._c), _ref(shape), None if e is None else _ref(e),
                            None if out is None else out.data_ptr(), None if q is None else _ref(q._c)), "yl_mx_conv2d")
+    _written(given)
     return q if want == "mx" else (out, q) if want == "both" else out
