@@ -468,7 +468,8 @@ float yl_entropy_from_histogram(const uint32_t *counts, int max_bin, float bin_w
  *  Every entry takes the device its pointers belong to and a stream of that device (hipStream_t as void *, NULL = the
  *  default stream), is asynchronous on it, leaves the caller's current device as it was, keeps no state between calls and
  *  allocates nothing, so calls from several threads, streams and captured graphs do not meet.  All data pointers are device
- *  memory.  A call that returns an error has launched nothing.
+ *  memory.  A call refused for its arguments (YL_ERR_ARG) has launched nothing; YL_ERR_DEVICE is an error of the device or of a
+ *  launch of this very call (what an earlier HIP call of the thread left to hipGetLastError is not reported).
  * ------------------------------------------------------------------ */
 
 /* element types of the ordinary tensors these entries read and write */

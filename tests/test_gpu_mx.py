@@ -522,6 +522,33 @@ def test_the_current_device_stays(mx):
     assert torch.cuda.current_device() == before
 
 
+def test_an_error_that_another_call_left_is_not_this_calls(mx):
+    """A HIP call of the thread fails and nobody has asked for its error yet: the operators work, report nothing, and leave it there."""
+    from yolo2_light_amd._lib import lib
+    w, _ = make(mx, 300, 64, 1)
+    x = rand(200, 64, seed=2).cuda()
+    f, img = mx.quantize_filters(rand(8, 64, 1, 1, seed=3).cuda()), rand(1, 64, 5, 5, seed=4).cuda()
+    q, qi, y, y1 = mx.quantize(x), mx.quantize_nchw(img), mx.linear(x, w), mx.linear(x[:1], w)
+    v, c = mx.dequantize(q), mx.conv2d(qi, f, 1, 5, 5, 1)
+    got = [torch.zeros_like(t) for t in (y, y1, v, c)]
+    spare, q2 = torch.empty(200 * 4 * 17, dtype=torch.uint8, device="cuda"), mx.Matrix.empty(200, 64, "cuda")
+    del spare                                                     # the allocator holds linear's workspace
+    torch.cuda.synchronize()
+    lib.hipGetLastError()
+    try:
+        assert lib.hipSetDevice(4096) != 0                        # no such device: refused, and kept as the thread's last error
+        kept = lib.hipPeekAtLastError()
+        mx.quantize(x, out=q2)
+        mx.linear(x, w, out=got[0])
+        mx.linear(x[:1], w, out=got[1])
+        mx.dequantize(q2, out=got[2])
+        mx.conv2d(qi, f, 1, 5, 5, 1, out=got[3])
+        assert lib.hipPeekAtLastError() == kept
+    finally:
+        lib.hipGetLastError()
+    assert all(torch.equal(a, b) for a, b in zip(got, (y, y1, v, c)))
+
+
 def test_offsets_beyond_32_bits(mx):
     """Inputs, codes and results whose byte offsets pass 2^32: the last rows are as right as the first."""
     rows, k = 66_000, 33_000

@@ -3,11 +3,30 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
+#include <tuple>
+#include <utility>
 
 #include "../../include/yolo2_hip.h"
 #include "activations.h"
 
 namespace yl {
+
+// A launch and its own status.  (hipGetLastError behind it would also report what an earlier call of the thread, another library's
+// included, left there.)  A launch counts its threads in 32 bits.
+template <typename... P, size_t... I>
+inline int mx_launch_with(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t s, std::tuple<P...> values, std::index_sequence<I...>)
+{
+    if ((uint64_t)grid.x * block.x > 0xFFFFFFFFull) return (int)hipErrorInvalidConfiguration;
+    void *args[] = {&std::get<I>(values)...};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, args, 0, s);
+    if (e != hipSuccess) (void)hipGetLastError();          // it is this call's answer, not one for the thread's next question
+    return (int)e;
+}
+template <typename... P, typename... A>
+inline int mx_launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t s, A... args)
+{
+    return mx_launch_with(kernel, grid, block, s, std::tuple<P...>(args...), std::index_sequence_for<P...>{});
+}
 
 typedef int mx_v4i __attribute__((ext_vector_type(4)));
 typedef int mx_v8i __attribute__((ext_vector_type(8)));

@@ -181,11 +181,10 @@ static int launch_few(const MxProductArgs &a, const MxDense &x, hipStream_t s)
 {
     const dim3 grid((unsigned)((a.J + C - 1) / C)), block(MX_FEW_THREADS);
     switch (a.type) {
-    case YL_F32: hipLaunchKernelGGL((mx_product_few_kernel<YL_F32, C, FUSED>), grid, block, 0, s, a, x); break;
-    case YL_F16: hipLaunchKernelGGL((mx_product_few_kernel<YL_F16, C, FUSED>), grid, block, 0, s, a, x); break;
-    default: hipLaunchKernelGGL((mx_product_few_kernel<YL_BF16, C, FUSED>), grid, block, 0, s, a, x); break;
+    case YL_F32: return mx_launch(mx_product_few_kernel<YL_F32, C, FUSED>, grid, block, s, a, x);
+    case YL_F16: return mx_launch(mx_product_few_kernel<YL_F16, C, FUSED>, grid, block, s, a, x);
+    default: return mx_launch(mx_product_few_kernel<YL_BF16, C, FUSED>, grid, block, s, a, x);
     }
-    return (int)hipGetLastError();
 }
 
 int launch_mx_few(const MxProductArgs &a, void *stream)

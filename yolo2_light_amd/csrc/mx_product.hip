@@ -513,8 +513,7 @@ static int launch_tile(const MxProductArgs &a, hipStream_t s)
     }
     const int64_t grid = (int64_t)d.tiles_i * d.tiles_j;
     if (grid > 0x7fffffffLL) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((mx_product_tile_kernel<TYPE, CONV, BYTES, RARE, TI, TJ>), dim3((unsigned)grid), dim3(MX_THREADS), 0, s, d);
-    return (int)hipGetLastError();
+    return mx_launch(mx_product_tile_kernel<TYPE, CONV, BYTES, RARE, TI, TJ>, dim3((unsigned)grid), dim3(MX_THREADS), s, d);
 }
 
 // The tile, measured on MI355X (GPU time, both sides of each border):

@@ -157,17 +157,16 @@ static int launch_quantize(const MxDense &src, void *codes, void *scales, int64_
     if (src.k_stride == 1 || src.k == 1) {
         const int64_t g = (n + 63) / 64;
         const dim3 grid((unsigned)(g > 1 << 20 ? 1 << 20 : g));
-        if (n < 0x60000000) hipLaunchKernelGGL((mx_quantize_rows_kernel<TYPE, unsigned>), grid, dim3(256), 0, s, src, (unsigned *)codes, (unsigned char *)scales, ld, (unsigned)kb, (unsigned)n);
-        else hipLaunchKernelGGL((mx_quantize_rows_kernel<TYPE, int64_t>), grid, dim3(256), 0, s, src, (unsigned *)codes, (unsigned char *)scales, ld, kb, n);
+        if (n < 0x60000000) return mx_launch(mx_quantize_rows_kernel<TYPE, unsigned>, grid, dim3(256), s, src, (unsigned *)codes, (unsigned char *)scales, ld, (unsigned)kb, (unsigned)n);
+        return mx_launch(mx_quantize_rows_kernel<TYPE, int64_t>, grid, dim3(256), s, src, (unsigned *)codes, (unsigned char *)scales, ld, kb, n);
     } else {
         const int64_t tiles = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS;
         const int blocks = columns_blocks(tiles, kb);
         const int64_t groups = (kb + blocks - 1) / blocks, g = tiles * groups;
         if (g > 0x7fffffff) return (int)hipErrorInvalidValue;
-        if (blocks == 8) hipLaunchKernelGGL((mx_quantize_columns_kernel<TYPE, 8>), dim3((unsigned)g), dim3(256), 0, s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
-        else hipLaunchKernelGGL((mx_quantize_columns_kernel<TYPE, 4>), dim3((unsigned)g), dim3(256), 0, s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
+        if (blocks == 8) return mx_launch(mx_quantize_columns_kernel<TYPE, 8>, dim3((unsigned)g), dim3(256), s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
+        return mx_launch(mx_quantize_columns_kernel<TYPE, 4>, dim3((unsigned)g), dim3(256), s, src, (uint4 *)codes, (unsigned char *)scales, ld, kb, groups);
     }
-    return (int)hipGetLastError();
 }
 
 template <int TYPE>
@@ -177,17 +176,16 @@ static int launch_dequantize(const void *codes, const void *scales, int64_t ld, 
     if (dst.k_stride == 1 || dst.k == 1) {
         const int64_t g = (n + 63) / 64;
         const dim3 grid((unsigned)(g > 1 << 20 ? 1 << 20 : g));
-        if (n < 0x60000000) hipLaunchKernelGGL((mx_dequantize_rows_kernel<TYPE, unsigned>), grid, dim3(256), 0, s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, (unsigned)kb, (unsigned)n);
-        else hipLaunchKernelGGL((mx_dequantize_rows_kernel<TYPE, int64_t>), grid, dim3(256), 0, s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, kb, n);
+        if (n < 0x60000000) return mx_launch(mx_dequantize_rows_kernel<TYPE, unsigned>, grid, dim3(256), s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, (unsigned)kb, (unsigned)n);
+        return mx_launch(mx_dequantize_rows_kernel<TYPE, int64_t>, grid, dim3(256), s, (const unsigned *)codes, (const unsigned char *)scales, ld, dst, kb, n);
     } else {
         const int64_t tiles = (rows + MX_COLS_ROWS - 1) / MX_COLS_ROWS;
         const int blocks = columns_blocks(tiles, kb);
         const int64_t groups = (kb + blocks - 1) / blocks, g = tiles * groups;
         if (g > 0x7fffffff) return (int)hipErrorInvalidValue;
-        if (blocks == 8) hipLaunchKernelGGL((mx_dequantize_columns_kernel<TYPE, 8>), dim3((unsigned)g), dim3(256), 0, s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
-        else hipLaunchKernelGGL((mx_dequantize_columns_kernel<TYPE, 4>), dim3((unsigned)g), dim3(256), 0, s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
+        if (blocks == 8) return mx_launch(mx_dequantize_columns_kernel<TYPE, 8>, dim3((unsigned)g), dim3(256), s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
+        return mx_launch(mx_dequantize_columns_kernel<TYPE, 4>, dim3((unsigned)g), dim3(256), s, (const uint4 *)codes, (const unsigned char *)scales, ld, dst, kb, groups);
     }
-    return (int)hipGetLastError();
 }
 
 int launch_mx_quantize(const MxDense &src, void *codes, void *scales, int64_t ld, void *stream)
