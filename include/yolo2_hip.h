@@ -480,8 +480,8 @@ enum { YL_F32 = 0, YL_F16 = 1, YL_BF16 = 2 };
  *                                       low half of byte i, value 2i + 1 in the high half
  *   scales[r * ld + j]                  E8M0: the block's values are code * 2^(scale - 127); 255 = every value of the block is NaN
  * ld >= ceil(k / 32) is the row stride in blocks (a multiple of 4 keeps rows on 64 bytes and lets kernels load scales by words).
- * Where k % 32 != 0 the codes behind k in a row's last block are zero.  Blocks from ceil(k / 32) to ld are neither read nor written.
- * codes must be 16-byte aligned. */
+ * Where k % 32 != 0 the codes behind k in a row's last block are zero.  Blocks from ceil(k / 32) to ld count for nothing and are not
+ * written; their codes are not read, their scale bytes may be (scales travel in aligned words of four).  codes must be 16-byte aligned. */
 typedef struct yl_mx_matrix {
     void *codes, *scales;
     int64_t rows, k, ld;
@@ -518,10 +518,10 @@ int yl_mx_quantize(int device, void *stream, const yl_dense *src, const yl_mx_ma
 int yl_mx_dequantize(int device, void *stream, const yl_mx_matrix *src, const yl_dense *dst);
 
 /* y[m][n] = activate(sum over k of x[m][k] * w[n][k] + bias[n]) + residual[m][n], summed in 32 bits.
- * y: batch 1, rows = x->rows, k = w->rows, k_stride 1; it may not overlap the operands (beside them in the same rows is well). */
+ * y: batch 1, rows = x->rows, k = w->rows, k_stride 1; it may not overlap the operands. */
 int yl_mx_matmul(int device, void *stream, const yl_mx_matrix *x, const yl_mx_matrix *w, const yl_mx_epilogue *epilogue, const yl_dense *y);
 
-/* yl_mx_matmul on yl_mx_quantize(x), the same bits, in one call.  x: batch 1.  `workspace` is device memory of at least
+/* yl_mx_matmul on yl_mx_quantize(x), the same bits, in one call.  x: batch 1; y may lie beside it in the same rows.  `workspace` is device memory of at least
  * yl_mx_linear_workspace(x->rows, x->k) bytes, 16-byte aligned, which holds the rounded x while the call runs: calls that may run
  * at the same time need one each.  (It is 0 where the product rounds x itself -- a few rows, the single token of a decoding step -- and
  * for an x of more than 2^46 blocks, which yl_mx_linear refuses.) */
