@@ -469,7 +469,8 @@ float yl_entropy_from_histogram(const uint32_t *counts, int max_bin, float bin_w
  *  default stream), is asynchronous on it, leaves the caller's current device as it was, keeps no state between calls and
  *  allocates nothing, so calls from several threads, streams and captured graphs do not meet.  All data pointers are device
  *  memory.  A call refused for its arguments (YL_ERR_ARG) has launched nothing; YL_ERR_DEVICE is an error of the device or of a
- *  launch of this very call (what an earlier HIP call of the thread left to hipGetLastError is not reported).
+ *  launch of this very call (what an earlier HIP call of the thread left to hipGetLastError is not reported).  Sizes whose launch would count
+ *  more than 2^32 threads are refused: 2^27 rows of w and more under a few rows of x, 2^30 rows whose k is not contiguous to be rounded.
  * ------------------------------------------------------------------ */
 
 /* element types of the ordinary tensors these entries read and write */

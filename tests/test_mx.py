@@ -258,6 +258,37 @@ def test_as_many_rows_as_32_bits_count():
         refused(matmul(x={**x, "codes": 1 << 40, "scales": 1 << 43}, w=w, y=y), "2^31 - 257")
 
 
+FAR = dict(codes=1 << 45, scales=1 << 50)
+
+
+@pytest.mark.skipif(HAVE_GPU, reason="asks the entries for sizes without memory behind them: ends at the missing device")
+def test_launches_of_more_than_32_bits_of_threads():
+    """Every form at the largest size it launches, and one workgroup above it."""
+    def both(call, most):
+        accepted(call(most))
+        refused(call(most + 1), "2^32 threads")
+    # rounding tensors whose k is not contiguous: 64 rows by up to 8 blocks a workgroup of 256
+    for k, groups in ((2, 1), (256, 1), (257, 2), (4096, 16)):
+        most = (2 ** 24 - 1) // groups * 64
+        both(lambda rows: quantize(dense(rows=rows, k=k, rs=1, ks=1 << 31, data=1 << 54), matrix(rows=rows, k=k, ld=(k + 31) // 32, **FAR)), most)
+        both(lambda rows: dequantize(matrix(rows=rows, k=k, ld=(k + 31) // 32, **FAR), dense(rows=rows, k=k, rs=1, ks=1 << 31, data=1 << 54)), most)
+        accepted(quantize(dense(rows=1 << 31, k=k, data=1 << 54), matrix(rows=1 << 31, k=k, ld=(k + 31) // 32, **FAR)))         # contiguous k: a loop
+    w = lambda rows: dict(rows=rows, k=32, ld=1, **FAR)  # noqa: E731
+    y = lambda m, n: dict(rows=m, k=n, data=1 << 53)  # noqa: E731
+    for m, most in ((1, (2 ** 23 - 1) * 16), (16, (2 ** 23 - 1) * 16), (17, (2 ** 23 - 1) * 32), (32, (2 ** 23 - 1) * 32)):      # 512 threads a workgroup
+        both(lambda n: matmul(x=dict(rows=m, k=32, ld=1), w=w(n), y=y(m, n)), most)
+        both(lambda n: linear(x=dense(rows=m, k=32), w=w(n), y=y(m, n)), most)
+    accepted(matmul(x=dict(rows=33, k=32, ld=1), w=w(2 ** 31 - 257), y=y(33, 2 ** 31 - 257)))
+    rare = MxEpilogue(None, 0, None, 0)                           # 64 x 64 tiles alone
+    both(lambda n: matmul(x=dict(rows=64, k=32, ld=1), w=w(n), y=y(64, n), e=rare), (2 ** 24 - 1) * 64)
+    most = (2 ** 24 - 1) * 64                                     # x in columns of a workspace
+    both(lambda m: linear(x=dense(rows=m, k=32, rs=1, ks=1 << 31, data=1 << 40), w=dict(rows=1, k=32, ld=1), y=y(m, 1), ws=1 << 57, ws_bytes=1 << 40), most)
+    most = (2 ** 24 - 1) * 64 // 2 ** 12                          # images of 64 x 64
+    x = lambda b: matrix(rows=b * 4096, k=32, ld=1, **FAR)  # noqa: E731
+    f = matrix(rows=8, k=32, ld=1)
+    both(lambda b: conv(x=x(b), f=f, shape=(b, 64, 64, 1, 1, 0), e=rare, out=1 << 57), most)
+
+
 def test_no_such_device():
     for device in (-1, 4096):
         rc = quantize(dense(), matrix(), device=device)

@@ -3,6 +3,8 @@
 #include <cstdint>
 #include <cstddef>
 
+#include "../../include/yolo2_hip.h"
+
 namespace yl {
 
 constexpr int MX_BLOCK = 32;       // values a scale covers; 16 bytes of codes
@@ -65,8 +67,26 @@ int launch_mx_product(const MxProductArgs &a, void *stream, char *name = nullptr
 // few rows (mx_few.hip)
 bool mx_few_takes(int64_t rows);
 int launch_mx_few(const MxProductArgs &a, void *stream);
+// an activation other than LINEAR, LEAKY and RELU
+inline bool mx_rare(int act) { return act != YL_LINEAR && act != YL_LEAKY && act != YL_RELU; }
 // the linear layer on an ordinary x (launch_mx_product's a_codes / a_scales / a_ld unused), where mx_linear_fused(rows, k)
 bool mx_linear_fused(int64_t rows, int64_t k);
 int launch_mx_linear(const MxProductArgs &a, const MxDense &x, void *stream);
+
+// Whether a launch's threads are counted in 32 bits, for the form that a call of such a size takes (above 2^20 workgroups none depends on
+// the number of CUs any more).  Rounding: only tensors whose k is not contiguous have a workgroup for every 64 rows.
+constexpr int64_t MX_MAX_THREADS = 0xFFFFFFFFLL;
+inline bool mx_rounding_fits(const MxDense &t)
+{
+    const int64_t kb = (t.k + MX_BLOCK - 1) / MX_BLOCK;
+    return t.k_stride == 1 || t.k <= 1 || t.batch * t.rows <= 0 || (t.batch * t.rows + 63) / 64 <= MX_MAX_THREADS / 256 / ((kb + 7) / 8);
+}
+inline bool mx_product_fits(const MxProductArgs &a)
+{
+    auto tiles = [&](int64_t ti, int64_t tj) { return ((a.I + ti - 1) / ti) * ((a.J + tj - 1) / tj); };
+    if (!a.conv && mx_few_takes(a.I)) return tiles(32, a.I <= 16 && mx_linear_fused(a.I, a.k) ? 16 : 32) <= MX_MAX_THREADS / 512;
+    const int64_t n = mx_rare(a.act) ? tiles(64, 64) : a.conv ? tiles(64, 128) : a.kb >= 64 ? tiles(256, 256) : tiles(128, 128);
+    return n <= MX_MAX_THREADS / 256;
+}
 
 }  // namespace yl

@@ -9,6 +9,7 @@
 namespace yl {
 namespace {
 
+constexpr const char *MX_TOO_MANY = "more than 2^32 threads in a launch";
 constexpr int64_t MX_MAX_LD = (int64_t)1 << 19;           // blocks a row: 32-bit offsets inside a tile of 256 rows
 
 // nothing may be thrown through a C entry: an error text that finds no memory is left out
@@ -154,7 +155,7 @@ const char *check_product(int64_t x_rows, int64_t x_k, const yl_mx_matrix *w, co
     a->bias = e ? e->bias : nullptr; a->act = e ? e->activation : YL_LINEAR;
     a->residual = e ? e->residual : nullptr; a->residual_stride = e ? e->residual_stride : 0;
     a->out = y->data; a->out_stride = y->row_stride; a->type = y->type;
-    return nullptr;
+    return mx_product_fits(*a) ? nullptr : MX_TOO_MANY;
 }
 
 }  // namespace
@@ -179,6 +180,7 @@ int yl_mx_quantize(int device, void *stream, const yl_dense *src, const yl_mx_ma
     const Range r = dense_range(src), c = codes_range(dst), s = scales_range(dst);
     if (r.meets(c) || r.meets(s)) return refuse(entry, "dst overlaps src");
     if (c.meets(s)) return refuse(entry, "codes and scales overlap");
+    if (!mx_rounding_fits(dense_of(src))) return refuse(entry, MX_TOO_MANY);
     DeviceScope scope;
     if (int rc = scope.enter(entry, device)) return rc;
     return launched(entry, launch_mx_quantize(dense_of(src), dst->codes, dst->scales, dst->ld, stream));
@@ -193,6 +195,7 @@ int yl_mx_dequantize(int device, void *stream, const yl_mx_matrix *src, const yl
     if (src->k != dst->k || src->rows != dst->batch * dst->rows) return refuse(entry, "dst is not src's rows by k");
     const Range r = dense_range(dst);
     if (r.meets(codes_range(src)) || r.meets(scales_range(src))) return refuse(entry, "dst overlaps src");
+    if (!mx_rounding_fits(dense_of(dst))) return refuse(entry, MX_TOO_MANY);
     DeviceScope scope;
     if (int rc = scope.enter(entry, device)) return rc;
     return launched(entry, launch_mx_dequantize(src->codes, src->scales, src->ld, dense_of(dst), stream));
@@ -234,6 +237,7 @@ int yl_mx_linear(int device, void *stream, const yl_dense *x, const yl_mx_matrix
     const bool fused = mx_linear_fused(x->rows, x->k), some = x->rows > 0 && x->k > 0;
     const int64_t need = yl_mx_linear_workspace(x->rows, x->k);
     if (some && !fused && need == 0) return refuse(entry, "x is too large for a workspace");
+    if (need > 0 && !mx_rounding_fits(dense_of(x))) return refuse(entry, MX_TOO_MANY);
     if (need > 0) {
         if (!workspace || workspace_bytes < need) return refuse(entry, "workspace is smaller than yl_mx_linear_workspace(x->rows, x->k)");
         if ((uintptr_t)workspace % 16) return refuse(entry, "workspace is not 16-byte aligned");
@@ -295,9 +299,6 @@ int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
         if (qr[0].meets(qr[1])) return refuse(entry, "codes and scales overlap");
         a.q_codes = q_out->codes; a.q_scales = q_out->scales; a.q_ld = q_out->ld;
     }
-    DeviceScope scope;
-    if (int rc = scope.enter(entry, device)) return rc;
-    if (!out && !q_out) return YL_OK;
     a.a_codes = filters->codes; a.a_scales = filters->scales; a.a_ld = filters->ld;
     a.b_codes = x->codes; a.b_scales = x->scales; a.b_ld = x->ld;
     a.I = I; a.J = J; a.kb = blocks_of(filters->k);
@@ -305,6 +306,10 @@ int yl_mx_conv2d(int device, void *stream, const yl_mx_matrix *x, const yl_mx_ma
     a.out = out; a.type = YL_F32;
     a.conv = true;
     a.H = c.h; a.W = c.w; a.OH = oh; a.OW = ow; a.G = (int)blocks_of(x->k); a.size = c.size; a.stride = c.stride; a.pad = c.pad; a.batch = c.batch;
+    if (!mx_product_fits(a)) return refuse(entry, MX_TOO_MANY);
+    DeviceScope scope;
+    if (int rc = scope.enter(entry, device)) return rc;
+    if (!out && !q_out) return YL_OK;
     return launched(entry, launch_mx_product(a, stream));
 }
 

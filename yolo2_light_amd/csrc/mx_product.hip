@@ -532,7 +532,7 @@ static int launch_by_size(const MxProductArgs &a, hipStream_t s, char *name, siz
 {
     auto grid = [&](int64_t ti, int64_t tj) { return (a.I + 64 * ti - 1) / (64 * ti) * ((a.J + 64 * tj - 1) / (64 * tj)); };
     const int64_t cus = device_cu_count();
-    const bool rare = a.act != YL_LINEAR && a.act != YL_LEAKY && a.act != YL_RELU;
+    const bool rare = mx_rare(a.act);
     int t = 11;
     if (!rare) {
         if (CONV) t = grid(1, 2) >= 2 * cus ? 12 : 11;
