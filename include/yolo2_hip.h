@@ -501,7 +501,9 @@ typedef struct yl_dense {
 /* what follows a product: y = activate(sum + bias[n]) + residual, in 32 bits, rounded once to y's type */
 typedef struct yl_mx_epilogue {
     const float *bias;          /* one a column of w / filter, or NULL */
-    int activation;             /* YL_LINEAR, YL_LEAKY, ... (any activation of this header) */
+    int activation;             /* YL_LINEAR, YL_LEAKY, ... (any activation of this header).  RELU is x * (x > 0) as everywhere in this
+                                   library: NaN of -Inf.  LEAKY is one product by 0.1f in 32 bits, up to an ulp from the .1 * x in
+                                   64 bits of the network's other convolutions */
     const void *residual;       /* y's type and shape, or NULL; may be y itself or lie beside it in the same rows, may not
                                    otherwise overlap it */
     int64_t residual_stride;    /* elements from row to row (the convolution: ignored, y's layout) */

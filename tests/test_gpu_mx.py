@@ -203,6 +203,98 @@ def test_products_that_fill_the_chip(mx, m, n, k, dtype):
     assert ((y - want).abs() <= tol).all(), ((y - want).abs() - tol).max()
 
 
+def whole_product_tolerance(x, w, bias, act, res, dtype, steps_of):
+    """mx_oracle.product_tolerance in FP64 on the GPU: activation(x w^T + bias) + res and how far a result may be from it."""
+    v = x @ w.t()
+    tol = ((o.blocks(steps_of) + 1) // 2 + 16) * 2.0 ** -23 * (x.abs() @ w.abs().t())
+    v = v + bias.double()
+    tol = tol + 2.0 ** -24 * (v.abs() + tol)
+    y = {"linear": lambda: v, "leaky": lambda: torch.where(v > 0, v, 0.1 * v), "relu": lambda: v.clamp(min=0), "logistic": lambda: torch.sigmoid(v)}[act]()
+    tol = 1.1 * tol + (2.0 ** -23 * y.abs() + 2.0 ** -24 if act != "linear" else 0)
+    if res is not None:
+        y = y + res.double()
+        tol = tol + 2.0 ** -24 * (y.abs() + tol)
+    half, least = o.HALF_STEP[dtype]
+    return y, tol + half * (y.abs() + tol) + least
+
+
+def random_matrix(mx, rows, k, seed, ld=None):
+    """Rows of every block different: random codes and scales over 2^5, what lies behind k's last block anything."""
+    g, kb = torch.Generator(device="cuda").manual_seed(seed), (k + 31) // 32
+    ld = ld or (kb + 3) // 4 * 4
+    codes = torch.randint(0, 256, (rows, 16 * ld), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.randint(120, 125, (rows, ld), dtype=torch.uint8, device="cuda", generator=g)
+    if k % 32:                                                    # the codes behind k in the last block are zero
+        last = codes[:, 16 * (kb - 1):16 * kb]
+        last[:, (k % 32 + 1) // 2:] = 0
+        if k % 2:
+            last[:, k % 32 // 2] &= 15
+    scales[:, kb:] = 255
+    return mx.Matrix(codes, scales, k)
+
+
+# (form, m, n, k, ld of x, ld of w): 256 x 256, 128 x 128, 64 x 128 and 64 x 64 tiles with scales by words and by bytes; k ends inside a panel of 256,
+# inside a word of four blocks and inside a block; rows and columns end inside a tile, in one and in both halves of it
+FORMS = [("256", 4100, 4099, 2100, 68, 68), ("256", 4096, 4352, 2048, 64, 64), ("256", 3841, 4330, 2177, 72, 72), ("256 bytes", 4100, 4099, 2100, 67, 69), ("256 bytes", 4000, 4200, 2321, 73, 76),
+         ("128", 3001, 2900, 1025, 36, 36), ("128 bytes", 3001, 2900, 1025, 33, 35), ("128, k >= 2048", 2000, 2100, 2100, 68, 68), ("128 bytes, k >= 2048", 2000, 2100, 2100, 66, 67),
+         ("64 x 128", 1000, 2500, 700, 24, 24), ("64 x 128 bytes", 1000, 2500, 700, 22, 25), ("64", 650, 700, 300, 12, 12), ("64 bytes", 650, 700, 300, 10, 11)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("form, m, n, k, x_ld, w_ld", FORMS, ids=["-".join(str(v) for v in f) for f in FORMS])
+def test_every_tile_with_the_whole_epilogue(mx, form, m, n, k, x_ld, w_ld, dtype):
+    """Every element of products that fill the chip: bias, activation, a residual and a result in rows of other lengths."""
+    x, w = random_matrix(mx, m, k, m, x_ld), random_matrix(mx, n, k, n + 1, w_ld)
+    bias = rand(n, seed=4).cuda()
+    res = rand(m, n + 5, seed=3, dtype=dtype).cuda()[:, 2:n + 2]
+    act = {"float32": "leaky", "float16": "relu", "bfloat16": "leaky"}[dtype]
+    whole = torch.full((m + 2, n + 9), 3.0, dtype=TYPES[dtype], device="cuda")
+    mx.matmul(x, w, bias=bias, activation=act, residual=res, out=whole[1:m + 1, 4:n + 4])
+    want, tol = whole_product_tolerance(gpu_values(mx, x), gpu_values(mx, w), bias, act, res, dtype, k)
+    off = (whole[1:m + 1, 4:n + 4].double() - want).abs() - tol
+    assert (off <= 0).all(), (off.max(), (off > 0).nonzero()[:4])
+    assert (whole[0] == 3).all() and (whole[m + 1] == 3).all() and (whole[:, :4] == 3).all() and (whole[:, n + 4:] == 3).all()
+    if dtype == "float32":                                        # the same sums without anything behind them
+        y = mx.matmul(x, w)
+        want, tol = whole_product_tolerance(gpu_values(mx, x), gpu_values(mx, w), torch.zeros_like(bias), "linear", None, dtype, k)
+        assert ((y.double() - want).abs() <= tol).all()
+        y = mx.matmul(x, w, bias=bias, activation="logistic", residual=res)        # 64 x 64 tiles, single values
+        want, tol = whole_product_tolerance(gpu_values(mx, x), gpu_values(mx, w), bias, "logistic", res, dtype, k)
+        assert ((y.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m", [1, 20, 40, 300])
+def test_stair(mx, m):
+    """The one activation with jumps: sums, bias and result are small multiples of 1/4, exact in FP32 and on whole numbers often."""
+    n, k = 70, 96
+    g = gen(m)
+    x, w = torch.randint(-3, 4, (m, k), generator=g).float() / 2, torch.randint(-1, 2, (n, k), generator=g).float() / 2
+    x[:, ::32], w[:, ::32] = 6.0, 4.0                             # scales of 1: every block holds the values as they are
+    bias = torch.randint(-20, 21, (n,), generator=g).float() / 4 - 60.0
+    xq, wq = mx.quantize(x.cuda()), mx.quantize(w.cuda())
+    assert (f64(mx.dequantize(xq)) == f64(x)).all() and (f64(mx.dequantize(wq)) == f64(w)).all()
+    v = f64(x) @ f64(w).T + f64(bias)
+    whole = np.floor(v)                                           # stair_activate: even steps are flat, odd ones rise
+    want = np.where(whole % 2 == 0, np.floor(v / 2), v - whole + np.floor(v / 2))
+    assert (v == whole).sum() > 10 and (v < 0).any() and (v > 0).any()
+    got = mx.matmul(xq, wq, bias=bias.cuda(), activation="stair")
+    assert (f64(got) == want).all()
+
+
+@pytest.mark.parametrize("m", [1, 16, 20, 40, 200])
+def test_activations_of_infinities(mx, m):
+    """RELU is x * (x > 0), here as in every path of this library: NaN of -Inf.  The others as their formulas say."""
+    n, k = 48, 64
+    big = mx.Matrix(torch.full((m, 64), 0x77, dtype=torch.uint8, device="cuda"), torch.full((m, 4), 254, dtype=torch.uint8, device="cuda"), k)
+    wc = torch.full((n, 64), 0x77, dtype=torch.uint8, device="cuda")
+    wc[n // 2:] = 0xFF                                            # -6: the sums of the upper half are -Inf
+    w = mx.Matrix(wc, torch.full((n, 4), 254, dtype=torch.uint8, device="cuda"), k)
+    inf, nan = float("inf"), float("nan")
+    for act, up, down in (("linear", inf, -inf), ("leaky", inf, -inf), ("relu", inf, nan), ("logistic", 1.0, 0.0), ("relie", inf, -inf), ("hardtan", 1.0, -1.0), ("lhtan", inf, -inf)):
+        want = torch.tensor([up] * (n // 2) + [down] * (n - n // 2), device="cuda").expand(m, n)
+        assert torch.equal(mx.matmul(big, w, activation=act).nan_to_num(12.5), want.nan_to_num(12.5)), act
+
+
 @pytest.mark.parametrize("m, n, k", [(1, 100, 200), (7, 33, 64), (40, 129, 300), (130, 260, 96), (300, 300, 300)])
 @pytest.mark.parametrize("act", ["leaky", "relu", "logistic", "tanh", "elu", "relie", "ramp", "hardtan", "lhtan", "plse", "loggy"])
 def test_epilogues(mx, m, n, k, act):
@@ -379,6 +471,23 @@ def test_convolutions(mx, batch, c, n, h, w, size, stride, pad):
     r2 = res.cuda()
     z = mx.conv2d(q, fq, batch, h, w, size, stride, pad, bias=bias.cuda(), activation="leaky", residual=r2, out=r2)      # in place
     assert torch.equal(z, y)
+
+
+@pytest.mark.parametrize("act", ["relu", "logistic", "tanh", "elu", "relie", "ramp", "hardtan", "lhtan", "plse", "loggy"])
+@pytest.mark.parametrize("batch, c, n, h, w, size, stride, pad", [(2, 64, 70, 9, 7, 3, 1, 1), (1, 33, 17, 6, 6, 3, 2, 1), (3, 128, 130, 13, 13, 1, 1, 0)])
+def test_convolutions_with_every_activation(mx, batch, c, n, h, w, size, stride, pad, act):
+    """... and their MXFP4 output, where filters end inside a block: what is behind them is zero, whatever the activation makes of zero."""
+    x, f, xv, fv, _ = conv_case(mx, batch, c, n, h, w, size, seed=c + n)
+    win, oh, ow = o.windows(xv, batch, h, w, size, stride, pad)
+    bias, res = rand(n, seed=1, spread=0.2), rand(batch, n, oh, ow, seed=2)
+    want, tol = o.product_tolerance(win, fv, f64(bias), act, f64(res).transpose(0, 2, 3, 1).reshape(-1, n), "float32")
+    lay = lambda a: a.reshape(batch, oh, ow, n).transpose(0, 3, 1, 2)  # noqa: E731
+    args = (mx.quantize_nchw(x), mx.quantize_filters(f), batch, h, w, size, stride, pad)
+    y, side = mx.conv2d(*args, bias=bias.cuda(), activation=act, residual=res.cuda(), want="both")
+    close(y, lay(want), lay(tol))
+    only = mx.conv2d(*args, bias=bias.cuda(), activation=act, residual=res.cuda(), want="mx")
+    for q in (side, only):
+        check_matrix(q, f64(y).transpose(0, 2, 3, 1).reshape(-1, n))
 
 
 @pytest.mark.parametrize("batch, c, n, h, w, size, stride, pad", [(8, 32, 300, 50, 51, 3, 1, 1), (4, 160, 512, 61, 40, 3, 1, 1), (16, 128, 256, 64, 70, 3, 2, 1),

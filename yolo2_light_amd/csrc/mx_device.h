@@ -91,7 +91,9 @@ __device__ __forceinline__ mx_u32x4 mx_load_vec(const void *p, int64_t i) { retu
 template <int TYPE>
 __device__ __forceinline__ void mx_store_vec(void *p, int64_t i, mx_u32x4 v) { *reinterpret_cast<mx_u32x4_any *>(reinterpret_cast<char *>(p) + i * (16 / MX_VEC<TYPE>)) = v; }
 
-// activate(): LINEAR, LEAKY and RELU (x * (x > 0)) by one slope below zero, in 32 bits; the others only where RARE says so
+// activate(): LINEAR, LEAKY and RELU (x * (x > 0): NaN of -Inf) by one slope below zero, in 32 bits; the others only where RARE says so.
+// LEAKY's product by 0.1f is off by 2^-24 (the rounding) + 2^-26 (0.1f) of the value at most; (float)(.1 * (double)x), the other
+// convolutions' LEAKY, by 2^-24, for three conversions and multiplies in 64 bits an element.
 template <bool RARE>
 __device__ __forceinline__ float mx_activate(float v, int act)
 {
