@@ -73,6 +73,66 @@ def test_networks_teacher_forced_and_fused(name, width, height, batch):
     plain.close(); fused.close()
 
 
+@pytest.mark.parametrize("act", ["logistic", "relu", "relie", "ramp", "tanh", "plse", "elu", "loggy", "hardtan", "lhtan"])
+def test_a_layer_of_any_activation(act):
+    """The rare ones are a pass of their own behind the product, RELU too."""
+    from yolo2_light_amd.mx import ACTIVATIONS
+    B, C, H, W, M = 2, 64, 9, 11, 70
+    rng = np.random.default_rng(ACTIVATIONS[act])
+    w0, b0 = rng.normal(0, 0.3, C * C).astype(np.float32), rng.normal(0, 0.1, C).astype(np.float32)
+    wts, bias = rng.normal(0, (2.0 / (C * 9)) ** 0.5, M * C * 9).astype(np.float32), rng.normal(0, 0.5, M).astype(np.float32)
+    net = Network.from_desc([D.conv(B, W, H, C, C, 1, 1, 0, D.LEAKY, w0, b0), D.conv(B, W, H, C, M, 3, 1, 1, ACTIVATIONS[act], wts, bias)], B, W, H, C)
+    net.set_precision(MXFP4)
+    net.to_device(0)
+    got = net.predict(rng.standard_normal((B, C, H, W)).astype(np.float32))
+    assert "mx_product" in net.layer_kernel(1)
+    rows = o.rounded(net.layer_output(0).reshape(B, C, H * W).transpose(0, 2, 1).reshape(-1, C))
+    win, oh, ow = o.windows(rows, B, H, W, 3, 1, 1)
+    want, tol = o.product_tolerance(win, o.rounded(o.filter_rows(wts.astype(np.float64).reshape(M, C, 3, 3))), bias.astype(np.float64), act, None, "float32")
+    lay = lambda a: a.reshape(B, oh * ow, M).transpose(0, 2, 1).reshape(-1)  # noqa: E731
+    assert (np.abs(got - lay(want)) <= lay(tol)).all()
+    net.close()
+
+
+def test_a_network_at_its_own_size():
+    """yolov3 at 608 x 608: its layers fill the chip in other tiles than the small maps above; some of every stage in 64 bits, fused == unfused."""
+    torch = pytest.importorskip("torch")
+    from yolo2_light_amd import mx
+    cfg, wts = common.model_files("yolov3", 608, 608)
+    batch = 2
+    x = common.seeded_input(batch, 3, 608, 608)
+    plain = Network.load(cfg, wts, batch, 0, device=0, mxfp4=True)
+    plain.predict(x)
+    infos, kernels = plain.layers(), set()
+    for i in (1, 2, 5, 7, 12, 13, 38, 63, 75, 87):
+        li = infos[i]
+        assert li["int8"] == 3
+        kernels.add(plain.layer_kernel(i))
+        c, n, size, h, w = li["c"], li["n"], li["size"], li["h"], li["w"]
+        src = torch.from_numpy(np.ascontiguousarray(plain.layer_output(i - 1).reshape(batch, c, h, w))).cuda()
+        f = torch.from_numpy(np.ascontiguousarray(plain.layer_weights(i).reshape(n, c, size, size))).cuda()
+        xv = mx.dequantize_nchw(mx.quantize_nchw(src), batch, h, w).double().cpu()            # compared with mx_oracle.py in test_gpu_mx.py
+        fv = mx.dequantize(mx.quantize_filters(f)).double().view(n, size, size, c).permute(0, 3, 1, 2).cpu()
+        del src, f
+        step = max(1, n // 32)                                    # every step-th filter, the last one too
+        some = sorted(set(range(0, n, step)) | {n - 1})
+        v = torch.nn.functional.conv2d(xv, fv[some], stride=li["stride"], padding=li["pad"])
+        tol = ((c // 32 * size * size + 1) // 2 + 16) * 2.0 ** -23 * torch.nn.functional.conv2d(xv.abs(), fv[some].abs(), stride=li["stride"], padding=li["pad"])
+        v = v + torch.from_numpy(plain.layer_biases(i).astype(np.float64))[some][None, :, None, None]
+        want = torch.where(v > 0, v, 0.1 * v)
+        tol = tol + 2.0 ** -22 * (v.abs() + tol) + 2.0 ** -24
+        got = torch.from_numpy(plain.layer_output(i).reshape(batch, n, li["out_h"], li["out_w"])[:, some].astype(np.float64))
+        assert ((got - want).abs() <= tol).all(), "layer %d" % i
+        print("layer %d" % i, flush=True)
+    assert any("64x128" in k for k in kernels) and any("64x64" in k for k in kernels), kernels
+    heads = {i: plain.layer_output(i).copy() for i, li in enumerate(infos) if li["type"] == common.YOLO}
+    plain.close()
+    fused = Network.load(cfg, wts, batch, 0, device=0, fuse=True, mxfp4=True)
+    fused.predict(x)
+    assert len(heads) == 3 and all(np.array_equal(fused.layer_output(i).view(np.uint32), h.view(np.uint32)) for i, h in heads.items())
+    fused.close()
+
+
 def test_batch_items_are_independent():
     cfg, wts = common.model_files("yolov3", 96, 96)
     x = common.seeded_input(3, 3, 96, 96)
