@@ -311,3 +311,27 @@ def test_python_counts_the_rows_of_empty_tensors():
     for shape in ((2, 3, 0), (2, 0, 3), (0, 3, 5), (3, 0), (0, 3), (2, 3, 4, 0), (2, 3, 4)):
         d = mx._rows_of(torch.zeros(shape), "x")
         assert (d.rows, d.k) == (int(np.prod(shape[:-1])), shape[-1]), shape
+
+
+def test_python_views_of_a_matrix_from_two_threads():
+    """codes and scales of Matrix.empty are made when they are asked for: a thread that asks while another is between the two finds them right."""
+    torch = pytest.importorskip("torch")
+    from yolo2_light_amd import mx
+
+    class Between(mx.Matrix):                                      # reads scales the moment the first of the two is set
+        __slots__ = ("seen",)
+
+        def __setattr__(self, name, value):
+            first = name in ("_codes", "_scales") and value is not None and not hasattr(self, "seen")
+            super().__setattr__(name, value)
+            if first and hasattr(self, "_c"):
+                object.__setattr__(self, "seen", None)
+                object.__setattr__(self, "seen", (self.codes, self.scales))
+
+    for ask in ("codes", "scales"):
+        m = Between.empty(3, 200, "cpu")
+        got = getattr(m, ask)
+        for codes, scales in ((m.codes, m.scales), m.seen):
+            assert codes.shape == (3, 128) and scales.shape == (3, 8)
+            assert codes.data_ptr() == m._c.codes and scales.data_ptr() == m._c.scales
+        assert got.data_ptr() == getattr(m._c, ask) and m.device == torch.device("cpu")

@@ -70,7 +70,7 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device
 
 class Matrix:
     """rows x k values in MXFP4: codes uint8 [rows, 16 * ld], scales uint8 [rows, ld], ld >= ceil(k / 32) blocks a row."""
-    __slots__ = ("k", "rows", "index", "_codes", "_scales", "_c")
+    __slots__ = ("k", "rows", "index", "_both", "_codes", "_scales", "_c")
 
     def __init__(self, codes, scales, k: int):
         self.index = _tensor(codes, "codes")
@@ -83,7 +83,7 @@ class Matrix:
             _fail("codes [rows, 16 * ld] and scales [rows, ld] are contiguous and of the same rows and blocks")
         if k < 0 or ld < (k + BLOCK - 1) // BLOCK:
             _fail("k = %d needs %d blocks, the matrix has %d" % (k, (k + BLOCK - 1) // BLOCK, ld))
-        self.rows, self._codes, self._scales = rows, codes, scales
+        self.rows, self._both, self._codes, self._scales = rows, None, codes, scales
         self._c = MxMatrix(codes.data_ptr(), scales.data_ptr(), rows, k, ld)
 
     @classmethod
@@ -93,29 +93,28 @@ class Matrix:
         self = cls.__new__(cls)
         both = torch.empty(rows * ld * 17, dtype=torch.uint8, device=device)
         at = both.data_ptr()
-        self.k, self.rows, self.index, self._codes, self._scales = k, rows, both.get_device(), both, None
+        self.k, self.rows, self.index, self._both, self._codes, self._scales = k, rows, both.get_device(), both, None, None
         self._c = MxMatrix(at, at + rows * ld * 16, rows, k, ld)
         return self
 
-    def _views(self):
-        both, n, ld = self._codes, self.rows * self._c.ld, self._c.ld
-        self._codes, self._scales = both[:16 * n].view(self.rows, 16 * ld), both[16 * n:].view(self.rows, ld)
-
+    # views of the allocation, made when they are asked for; each by itself, so that threads that ask at once get the same ones
     @property
     def codes(self):
-        if self._scales is None:
-            self._views()
-        return self._codes
+        view = self._codes
+        if view is None:
+            view = self._codes = self._both[:16 * self.rows * self._c.ld].view(self.rows, 16 * self._c.ld)
+        return view
 
     @property
     def scales(self):
-        if self._scales is None:
-            self._views()
-        return self._scales
+        view = self._scales
+        if view is None:
+            view = self._scales = self._both[16 * self.rows * self._c.ld:].view(self.rows, self._c.ld)
+        return view
 
     @property
     def device(self):
-        return self._codes.device
+        return (self._codes if self._both is None else self._both).device
 
 
 def _written(*tensors):
@@ -169,7 +168,7 @@ def _quantize(src: Dense, device: int, out: Optional[Matrix]) -> Matrix:
         _matrix(q, "out", device)
     check(lib.yl_mx_quantize(device, _stream(device), _ref(src), _ref(q._c)), "yl_mx_quantize")
     if out is not None:
-        _written(out._codes, out._scales)
+        _written(out._both, *((out._codes, out._scales) if out._both is None else ()))
     return q
 
 
