@@ -7,9 +7,10 @@
 // order of the waves (the same bits every time), then bias, activation, residual, store.
 // FUSED (up to 16 rows): x is an ordinary tensor and every workgroup rounds all of it into its LDS while its first weights travel: no
 // launch and no workspace for the rounding, and the same codes and the same sums as rounding first.
-// MI355X: 1 x 4096 x 4096 from BF16 3.9 us (w alone at 5.1 TB/s: 1.7 us, the rest is the launch and one round trip to memory; three waits of
-// four cycles), 1 x 8192 x 8192 8.7 us (7.0), 32 x 8192 x 8192 12.4.  More rows lie with the tiles of mx_product.hip: every workgroup
-// here reads all of x, and at 64 rows that costs more than w (8192 x 8192: 18.3 us against 14.7).
+// MI355X: 1 x 4096 x 4096 from BF16 3.9 to 4.4 us (w alone at 5.1 TB/s: 1.7 us, the rest is the launch and one round trip to memory; three waits of
+// four cycles), 1 x 8192 x 8192 8.7 us (7.0), 32 x 8192 x 8192 12.6.  More rows lie with the tiles of mx_product.hip: every workgroup
+// here reads all of x, and at 64 rows that cost more than w (8192 x 8192, in a form for 64 rows: 18.3 us against 14.6).  At the border
+// 32 x 8192 x 8192 12.6 us against 13.6 with the tiles, 32 x 4096 x 4096 7.6 against 8.2, but 32 x 16384 x 4096 12.7 against 9.5.
 #include "activations.h"
 #include "mx_device.h"
 #include "mx.h"
@@ -27,8 +28,17 @@ static inline int64_t mx_few_lds(int64_t rows, int64_t k)
     return rows * ((kbp + 1) * 16 + kbp);
 }
 
-// Rounding x in every workgroup pays while it is little against the weights that travel meanwhile (MI355X, GPU time with / without it:
-// 4 x 4096 x 4096 5.9 us / 7.7, 8 x 4096 x 4096 7.9 / 7.9, 16 x 4096 x 4096 11.9 / 8.3), and saves the host a launch; one row always.
+// Rounding x in every workgroup pays while it is little against the weights that travel meanwhile, and saves the host a launch of 3 us; one row always.
+// MI355X, GPU time in us with it / with a launch of its own, k = 4096 (16 rows: k = 2048), by the rows of w:
+//   rows    1024         4096         16384         65536
+//   1       4.3 / 6.1    4.4 / 6.2    9.6 / 11.7    30.8 / 31.5     (k = 16384: 9.1 / 10.3, 10.1 / 11.2, 29.2 / 32.4, 117 / 129)
+//   2       4.8 / 6.2    4.9 / 6.4    10.9 / 11.5   36.4 / 31.4
+//   4       5.7 / 6.3    5.9 / 6.5    12.8 / 11.8   44.9 / 32.6
+//   8       7.7 / 6.6    8.0 / 6.7    19.0 / 12.2   63.9 / 32.3
+//   16      7.1 / 5.9    7.3 / 5.9    15.8 / 8.4    52.7 / 21.6
+//   16 rows of k = 4096, above the border: 11.6 / 7.1, 12.1 / 7.2, 29.9 / 13.1, 101 / 35
+// The rule sees rows and k alone (so does the workspace that a caller asks for): with up to 4096 rows of w the launch that it saves the
+// host is worth more than what it costs the GPU; with a w of many more rows and 8 to 16 rows of x it costs up to 2.5 times the time.
 bool mx_linear_fused(int64_t rows, int64_t k)
 {
     return rows <= 16 && k <= (int64_t)1 << 20 && (rows <= 1 || rows * k <= 32768) && mx_few_lds(rows, k) <= MX_FEW_LDS;
@@ -190,8 +200,8 @@ static int launch_few(const MxProductArgs &a, const MxDense &x, hipStream_t s)
 int launch_mx_few(const MxProductArgs &a, void *stream)
 {
     hipStream_t s = (hipStream_t)stream;
-    // 16 columns a workgroup where 32 would leave CUs without one (16 x 4096 x 4096 4.9 us against 6.6; 16 x 16384 x 4096 12.6 against
-    // 10.7), and where the fused form, which has no other, would run: its sums are these
+    // 16 columns a workgroup where 32 would leave CUs without one (16 x 4096 x 4096 5.0 us against 6.5; 16 x 16384 x 4096 12.5 against
+    // 10.6), and where the fused form, which has no other, would run: its sums are these
     if (a.I <= 16 && (a.J < 32 * (int64_t)device_cu_count() || mx_linear_fused(a.I, a.k))) return launch_few<16, false>(a, MxDense{}, s);
     return launch_few<32, false>(a, MxDense{}, s);
 }

@@ -6,7 +6,7 @@
 // of the same rows, each with its own scale byte -- exactly the format's block, so no code is ever unpacked.  Products of codes are
 // exact; the sum is FP32.  D's layout: lane l holds column l & 31, rows 8 (e / 4) + 4 (l >> 5) + e % 4.
 //
-// MI355X: 8192^3 280 to 292 us = 3.8 to 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
+// MI355X: 8192^3 285 to 300 us, by box = 3.7 to 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
 // but these instructions makes 9.2, four times the BF16 rate of a large library product 4.8.  At 256 x 256 the instructions are half of a
 // wave's cycles, a quarter are waits for panels out of L2 and at barriers.  One wave a tile with operands straight from memory, the
 // first form: 3.72 ms.
@@ -38,7 +38,7 @@ __device__ __forceinline__ mx_f32x16 mx_mfma(mx_v4i a, mx_v4i b, mx_f32x16 c, in
 }
 
 // A strip of D, 32 rows from ib by COLS columns from jb, in LDS: + bias, activation, + residual, to rows of memory.  WIDE: in 16-byte vectors,
-// wherever they begin (3420 x 15311 x 149 to BF16: 51 us by single values, which the rare activations are left with, 41 so), the
+// wherever they begin (3420 x 15311 x 149 to BF16: 51 us by single values, which the rare activations are left with, 36 to 41 so), the
 // last of a row by its values; INSIDE: no column is behind a row's end; AHEAD rows' addends are requested before the first is used.
 template <int TYPE, bool RARE, bool WIDE, bool INSIDE, int COLS, int PITCH>
 __device__ __forceinline__ void mx_finish_rows(const MxProductArgs &p, const float *strip, int ib, int jb, int lane)
@@ -138,7 +138,7 @@ __device__ __forceinline__ void mx_side_block(const MxProductArgs &p, int64_t j,
 
 // A convolution's 32 x 32 tile of D from registers to planes of memory.  `at`: byte offset of (this lane's position, row 0 of the image's
 // planes) in `out`; WHOLE: all 32 rows are filters.  This and the index arithmetic in front of the panels are most of a layer with few
-// channels: the bias comes as four vectors, rows are offsets of the instruction (76 x 76 256 -> 128 1x1 of 8 images 16.4 -> 10 us).
+// channels: the bias comes as four vectors, rows are offsets of the instruction (76 x 76 256 -> 128 1x1 of 8 images 16.4 -> 9.9 us, with the MXFP4 output alone 7.9).
 template <bool RARE, bool WHOLE>
 __device__ __forceinline__ void mx_finish_planes(const MxProductArgs &p, const mx_f32x16 &acc, int ib, int64_t j, bool ok, int half, __amdgpu_buffer_rsrc_t bias,
                                                  __amdgpu_buffer_rsrc_t out, __amdgpu_buffer_rsrc_t residual, int at)
@@ -517,16 +517,18 @@ static int launch_tile(const MxProductArgs &a, hipStream_t s)
 }
 
 // The tile, measured on MI355X (GPU time, both sides of each border):
-//   (both sides of a border from one build, whose epilogue took up to 15 % longer than this one's)
-//   rows    256 x 256 from k = 2048 on where it gives every CU a workgroup: 4096 x 16384 x 4096 185 us against 209 with 128 x 128 tiles, but
-//           4096 x 4096 x 1024 27.3 against 25.3 (one workgroup a CU hides neither end of a tile behind another)
-//           128 x 128 where it gives every CU two workgroups, or one from k = 2048 on: 512 x 8192 x 8192 31.1 us against 43.5 with 64 x 128
-//           tiles, 1024 x 4096 x 512 9.3 against 8.5
-//           64 x 128 where it gives every CU one (512 x 4096 x 4096 13.9 us against 16.4 with 128 x 128 and 14.3 with 64 x 64)
-//           else 64 x 64 (1024^3 5.6 us against 7.2 with 64 x 128)
+//   (BF16, replayed from a graph; both sides of a border from one build of this source with the tile forced, in turn)
+//   rows    256 x 256 from k = 2048 on where it gives every CU a workgroup: 4096 x 16384 x 4096 171 us against 206 with 128 x 128 tiles,
+//           4096 x 4096 x 2048 31.2 against 33.5, but 4096 x 4096 x 1024 24.3 against 22.9 (one workgroup a CU hides neither end of a tile behind another)
+//           128 x 128 where it gives every CU two workgroups, or one from k = 2048 on: 512 x 8192 x 8192 29.6 us against 38.7 with 64 x 128
+//           tiles, 2048 x 4096 x 512 11.5 against 12.3, but 1024 x 4096 x 512 8.2 against 7.8
+//           64 x 128 where it gives every CU one (512 x 4096 x 4096 13.2 us against 14.7 with 128 x 128 and 13.5 with 64 x 64)
+//           else 64 x 64 (1024^3 5.5 us against 6.8 with 64 x 128, 256 x 4096 x 4096 9.1 against 12.7)
 //   planes  64 x 128 where it gives every CU two workgroups, else 64 x 64: bound by the map's and the result's bytes and by the latency of
-//           gathering, they want waves (76 x 76 128 -> 256 3x3 of 64 images: 0.290 ms against 0.347 with 64 x 64; with 128 x 128 and 256 x 256
-//           1.1 and 1.9 times the time; 19 x 19 512 -> 1024 3x3 of 8 images 30 us with 64 x 64, 33.5 with 64 x 128)
+//           gathering, they want waves (76 x 76 128 -> 256 3x3 of 64 images: 190 us against 230 with 64 x 64, 240 with 128 x 128 and 1350 with
+//           256 x 256; 19 x 19 512 -> 1024 3x3 of 8 images 22.4 us with 64 x 64, 24.3 with 64 x 128; of 16 images 39.5 and 33.9)
+//   The activations other than LINEAR, LEAKY and RELU have 64 x 64 tiles and single stores only: 4096 x 16384 x 4096 with LOGISTIC 369 us,
+//   512 x 4096 x 4096 19.2, 3420 x 15311 x 149 123 (36 without).
 template <int TYPE, bool CONV, bool BYTES>
 static int launch_by_size(const MxProductArgs &a, hipStream_t s, char *name, size_t name_len)
 {

@@ -8,7 +8,8 @@
 //            wave reads 64 neighbouring pixels of a channel at a time; codes go through LDS, so that a row's blocks leave together
 // MI355X: 16 x 256 x 76 x 76 FP32 to MXFP4 and back 20.0 + 20.3 us, 6.0 TB/s (out of the 256 MB cache; 51 us from HBM, where a large copy
 // makes 5.1 TB/s); 4096 x 4096 BF16 rows 10.1 us; one row of 4096 2.3 us, which is a launch.  One thread a block with scalar loads, the
-// first form, took 52 us for the map's pair and 27 instead of 8.4 us for the pair on 3001 x 1005 FP16 values in rows of 1016.
+// first form, took 52 us for the map's pair and 27 instead of 7.1 us (both out of a graph; 4.4 + 4.1 each by itself) for the pair on
+// 3001 x 1005 FP16 values in rows of 1016.
 #include "mx_device.h"
 #include "mx.h"
 #include "kernels.h"
