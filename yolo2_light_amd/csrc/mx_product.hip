@@ -6,7 +6,7 @@
 // of the same rows, each with its own scale byte -- exactly the format's block, so no code is ever unpacked.  Products of codes are
 // exact; the sum is FP32.  D's layout: lane l holds column l & 31, rows 8 (e / 4) + 4 (l >> 5) + e % 4.
 //
-// MI355X: 8192^3 285 to 300 us, by box = 3.7 to 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
+// MI355X: 8192^3 285 to 300 us, by card = 3.7 to 3.9 PFLOP/s, 4.7 on the slope from k = 8192 to 16384, where the ends of the tiles no longer count; a loop of nothing
 // but these instructions makes 9.2, four times the BF16 rate of a large library product 4.8.  At 256 x 256 the instructions are half of a
 // wave's cycles, a quarter are waits for panels out of L2 and at barriers.  One wave a tile with operands straight from memory, the
 // first form: 3.72 ms.
