@@ -173,7 +173,8 @@ def _quantize(src: Dense, device: int, out: Optional[Matrix]) -> Matrix:
 
 
 def quantize(x, out: Optional[Matrix] = None) -> Matrix:
-    """x [..., k], any strides -> Matrix of x.numel() / k rows."""
+    """x [..., k] -> Matrix of one row a k-vector.  k and the rows may have any strides; more than one leading axis has to be one run of
+    equal steps (x.reshape(-1, k) without a copy)."""
     device = _tensor(x, "x")
     return _quantize(_rows_of(x, "x"), device, out)
 
